@@ -18,6 +18,7 @@ F32, BF16 = 0, 1
 PAD_ZERO, PAD_REFLECT = 0, 1
 FORM_GATHER, FORM_S2_TRANSPOSED = 0, 1
 CONV_ALONE = 1
+ACT_NONE, ACT_LRELU, ACT_SILU, ACT_GELU = 0, 1, 2, 3
 WS_HEADER = 40960        # floats of arrival counters at the start of a reduction workspace (CVG_WS_HEADER)
 
 
@@ -38,6 +39,21 @@ class WMap(C.Structure):
 class PackJob(C.Structure):
     _fields_ = [("map", WMap), ("canonical", C.c_void_p), ("packed", C.c_void_p), ("n_groups", C.c_int64)] + \
         [(n, C.c_int32) for n in ("block0", "mode", "rows", "ld", "nchunks", "ntaps", "Cin", "dtype")]
+
+
+class GnDesc(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("dtype", "B", "HW", "C", "G", "act", "x_ld", "res_ld", "y_ld", "dx_ld", "dres_ld")] + \
+        [("eps", C.c_float)]
+
+
+class LinearDesc(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("dtype", "M", "N", "K", "act", "dw_dtype", "x_ld", "w_ld", "y_ld", "res_ld", "pre_ld",
+                                         "dy_ld", "dx_ld", "dw_ld")]
+
+
+class DistillDesc(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("dtype", "R", "V", "top", "logits_ld", "dlogits_ld", "top_ld")] + \
+        [("temperature", C.c_float), ("grad_scale", C.c_float)]
 
 
 class CvgError(RuntimeError):
@@ -115,6 +131,13 @@ def _load():
                                                    vp, vp]),
         "cvg_gan_pair_feature_match": (C.c_int, [vp, i32, i32, i32, i32, i32, i32, f32, vp, vp, vp, vp]),
         "cvg_axpy_f32": (C.c_int, [vp, vp, f32, i64, vp]),
+        "cvg_gn_act_workspace": (sz, [P(GnDesc), i32]),
+        "cvg_gn_act_fwd": (C.c_int, [P(GnDesc), vp, vp, vp, vp, vp, vp, vp, sz, vp]),
+        "cvg_gn_act_bwd": (C.c_int, [P(GnDesc), vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]),
+        "cvg_linear_act_workspace": (sz, [P(LinearDesc), i32]),
+        "cvg_linear_act_fwd": (C.c_int, [P(LinearDesc), vp, vp, vp, vp, vp, vp, vp, sz, vp]),
+        "cvg_linear_act_bwd": (C.c_int, [P(LinearDesc), vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]),
+        "cvg_distill_topk": (C.c_int, [P(DistillDesc), vp, vp, vp, vp, vp, vp, vp, vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)          # AttributeError here = header and library disagree

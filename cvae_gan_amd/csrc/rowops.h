@@ -1,0 +1,67 @@
+// Helpers shared by the group-norm, linear and distillation kernels.
+#pragma once
+#include "common.h"
+
+// ---- activations (CVG_ACT_*) --------------------------------------------------------------------------------
+// SiLU and the tanh form of GELU are both v * sigmoid(a(v)): a = v, and a = 2 sqrt(2/pi) (v + 0.044715 v^3) because
+// 0.5 (1 + tanh u) = sigmoid(2u).  EXACT (f32 tensors): expf and an IEEE division; otherwise v_exp_f32 / v_rcp_f32,
+// whose one-ulp-scale errors sit sixteen bits below the bf16 rounding that follows.
+template <bool EXACT> __device__ __forceinline__ float fast_sigmoid(float a) {
+    if (EXACT) return 1.0f / (1.0f + expf(-a));
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(a * -1.4426950408889634f));
+}
+#define GELU_A 1.5957691216057308f       // 2 sqrt(2 / pi)
+#define GELU_B 0.044715f
+template <bool EXACT> __device__ __forceinline__ float act_value(float v, int act) {
+    switch (act) {
+        case CVG_ACT_LRELU: return v > 0.f ? v : LRELU_SLOPE * v;
+        case CVG_ACT_SILU: return v * fast_sigmoid<EXACT>(v);
+        case CVG_ACT_GELU: return v * fast_sigmoid<EXACT>(GELU_A * (v + GELU_B * v * v * v));
+        default: return v;
+    }
+}
+template <bool EXACT> __device__ __forceinline__ float act_slope(float v, int act) {
+    switch (act) {
+        case CVG_ACT_LRELU: return v > 0.f ? 1.f : LRELU_SLOPE;
+        case CVG_ACT_SILU: {
+            const float p = fast_sigmoid<EXACT>(v);
+            return p * (1.f + v * (1.f - p));
+        }
+        case CVG_ACT_GELU: {
+            // beyond |v| = 16 the slope is 0 or 1 to the last bit; the clamp keeps 0 * inf out of it (NaN passes: the
+            // comparisons are false for it)
+            const float c = v > 16.f ? 16.f : (v < -16.f ? -16.f : v);
+            const float p = fast_sigmoid<EXACT>(GELU_A * (c + GELU_B * c * c * c));
+            return p * (1.f + c * (1.f - p) * GELU_A * (1.f + 3.f * GELU_B * c * c));
+        }
+        default: return 1.f;
+    }
+}
+static inline bool act_known(int act) { return act >= CVG_ACT_NONE && act <= CVG_ACT_GELU; }
+
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+    return v;
+}
+static inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+// 8 elements as they lie in memory (registers that hold a tile between two passes)
+template <typename T> struct Raw8;
+template <> struct Raw8<bf16> { u32x4 a; };
+template <> struct Raw8<float> { u32x4 a, b; };
+__device__ __forceinline__ void raw_load(Raw8<bf16>& r, const bf16* p) { r.a = *(const u32x4*)p; }
+__device__ __forceinline__ void raw_load(Raw8<float>& r, const float* p) { r.a = *(const u32x4*)p; r.b = *(const u32x4*)(p + 4); }
+__device__ __forceinline__ void raw_zero(Raw8<bf16>& r) { r.a = u32x4{0, 0, 0, 0}; }
+__device__ __forceinline__ void raw_zero(Raw8<float>& r) { r.a = u32x4{0, 0, 0, 0}; r.b = r.a; }
+__device__ __forceinline__ void raw_f32(const Raw8<bf16>& r, float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(r.a[i] << 16);
+        v[2 * i + 1] = __uint_as_float(r.a[i] & 0xffff0000u);
+    }
+}
+__device__ __forceinline__ void raw_f32(const Raw8<float>& r, float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { v[i] = __uint_as_float(r.a[i]); v[4 + i] = __uint_as_float(r.b[i]); }
+}

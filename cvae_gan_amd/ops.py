@@ -7,8 +7,10 @@ import ctypes as C
 import torch
 
 from ._lib import lib, check, ConvDesc, WMap, PackJob, CvgError, F32, BF16, PAD_ZERO, PAD_REFLECT  # noqa: F401
+from ._lib import GnDesc, LinearDesc, DistillDesc, ACT_NONE, ACT_LRELU, ACT_SILU, ACT_GELU  # noqa: F401
 
 _DT = {torch.float32: F32, torch.bfloat16: BF16}
+ACTS = {"none": ACT_NONE, "lrelu": ACT_LRELU, "silu": ACT_SILU, "gelu": ACT_GELU}
 
 
 def dt(t_or_dtype):
@@ -323,3 +325,211 @@ def bn_eval_scale_shift(rm, rv, gamma, beta, C_, scale, shift):
 def conv_bn_act_fwd(desc, x, w, y, scale, shift, bias=None, cbias=None, labels=None, res=None):
     check(lib.cvg_conv_bn_act_fwd(C.byref(desc), ptr(x), ptr(w), ptr(y), ptr(bias), ptr(cbias), ptr(labels),
                                   ptr(scale), ptr(shift), ptr(res), stream()))
+
+
+# ---- group normalisation, fused linear layers, distillation ---------------------------------
+# Sizes and pitches come from the tensors; shapes, types, strides and devices are checked before anything is
+# launched (CvgError).  Kernels run on the current stream of the tensors' device.  A workspace is scratch for one call:
+# it may be reused by the next call on the same stream, calls that may overlap need their own; ws=None allocates one.
+def _need(ok, fmt, *args):
+    if not ok:
+        raise CvgError(fmt % args)
+
+
+def _like(name, t, ref_name, ref, shape=None, dtype=None):
+    """t (when given) has ref's device, and the given shape / dtype (default: ref's)."""
+    if t is None:
+        return
+    shape = ref.shape if shape is None else shape
+    dtype = ref.dtype if dtype is None else dtype
+    _need(tuple(t.shape) == tuple(shape), "%s has shape %s, expected %s", name, tuple(t.shape), tuple(shape))
+    _need(t.dtype == dtype, "%s is %s, expected %s", name, t.dtype, dtype)
+    _need(t.device == ref.device, "%s is on %s, %s on %s", name, t.device, ref_name, ref.device)
+
+
+def _dense(name, t):
+    _need(t is None or t.is_contiguous(), "%s has to be contiguous", name)
+
+
+def _pitch(name, t):
+    """Distance in elements between consecutive rows of the last dimension; all leading dimensions have to
+    enumerate rows at that one distance."""
+    if t is None or t.is_contiguous():
+        return 0
+    if t.numel() == 0:
+        return 0
+    width = t.shape[-1]
+    _need(width == 1 or t.stride(-1) == 1, "%s: the elements of a row have to be consecutive", name)
+    pitch, span = None, 1
+    for n, st in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+        if n == 1:
+            continue
+        if pitch is None:
+            pitch = st
+        _need(st == pitch * span, "%s: strides %s do not put the rows at one pitch", name, t.stride())
+        span *= n
+    if pitch is None:
+        return 0
+    _need(pitch >= width, "%s: rows of %d elements overlap at pitch %d", name, width, pitch)
+    _need(pitch < 2 ** 31, "%s: pitch %d", name, pitch)
+    return pitch
+
+
+def _launch(fn, dev, *args):
+    _need(dev.type == "cuda", "cvae_gan_amd ops need device tensors")
+    if dev.index == torch.cuda.current_device():
+        check(fn(*args, stream()))
+    else:
+        with torch.cuda.device(dev):
+            check(fn(*args, stream()))
+
+
+def _p(t):
+    return None if t is None else t.data_ptr()
+
+
+def _bytes(n, device):
+    return torch.empty(n, dtype=torch.uint8, device=device)
+
+
+def _nbytes(t):
+    return 0 if t is None else t.numel() * t.element_size()
+
+
+def _scratch(ws, n, device):
+    if ws is None:
+        return _bytes(n, device) if n else None
+    _need(ws.device == device and ws.is_contiguous(), "the workspace has to be contiguous on %s", device)
+    return ws
+
+
+def _gn_desc(x, G, act, eps=0.0):
+    _need(x.dim() >= 2 and x.dtype in _DT, "x has to be [B, ..., C] in float32 or bfloat16")
+    B, C_ = x.shape[0], x.shape[-1]
+    hw = 1
+    for n in x.shape[1:-1]:
+        hw *= n
+    _need(act in ACTS.values(), "activation %r", act)
+    d = GnDesc()
+    d.dtype, d.B, d.HW, d.C, d.G, d.act, d.eps = _DT[x.dtype], B, hw, C_, int(G), act, eps
+    return d
+
+
+def gn_act_workspace(x, G, backward=False):
+    """Workspace (a uint8 tensor) for gn_act_fwd on tensors like x, with backward also for gn_act_bwd."""
+    return _bytes(int(lib.cvg_gn_act_workspace(C.byref(_gn_desc(x, G, ACT_NONE)), int(backward))), x.device)
+
+
+def gn_act_fwd(x, res, y, G, stats, gamma, beta, eps=1e-5, act=ACT_LRELU, ws=None):
+    """y = act(groupnorm(x) * gamma + beta [+ res]); x, res, y [B, ..., C] channels last, stats f32 [2, B, G] (mean,
+    1 / std; None: not kept), gamma / beta f32 [C]."""
+    d = _gn_desc(x, G, act, eps)
+    _like("res", res, "x", x)
+    _like("y", y, "x", x)
+    for n, t in (("gamma", gamma), ("beta", beta)):
+        _like(n, t, "x", x, (d.C,), torch.float32)
+        _dense(n, t)
+    _like("stats", stats, "x", x, (2, d.B, d.G), torch.float32)
+    _dense("stats", stats)
+    d.x_ld, d.res_ld, d.y_ld = _pitch("x", x), _pitch("res", res), _pitch("y", y)
+    ws = _scratch(ws, 0 if ws is not None else int(lib.cvg_gn_act_workspace(C.byref(d), 0)), x.device)
+    _launch(lib.cvg_gn_act_fwd, x.device, C.byref(d), _p(x), _p(res), _p(y), _p(stats), _p(gamma), _p(beta), _p(ws), _nbytes(ws))
+
+
+def gn_act_bwd(dy, x, res, dx, dres, G, stats, gamma, beta, dgamma, dbeta, act=ACT_LRELU, ws=None):
+    """Gradients of gn_act_fwd: res as in the forward call, stats from it; dres may be None."""
+    d = _gn_desc(x, G, act)
+    for n, t in (("dy", dy), ("res", res), ("dx", dx), ("dres", dres)):
+        _like(n, t, "x", x)
+    for n, t in (("gamma", gamma), ("beta", beta), ("dgamma", dgamma), ("dbeta", dbeta)):
+        _like(n, t, "x", x, (d.C,), torch.float32)
+        _dense(n, t)
+    _like("stats", stats, "x", x, (2, d.B, d.G), torch.float32)
+    _dense("stats", stats)
+    d.x_ld, d.res_ld, d.y_ld = _pitch("x", x), _pitch("res", res), _pitch("dy", dy)
+    d.dx_ld, d.dres_ld = _pitch("dx", dx), _pitch("dres", dres)
+    ws = _scratch(ws, 0 if ws is not None else int(lib.cvg_gn_act_workspace(C.byref(d), 1)), x.device)
+    _launch(lib.cvg_gn_act_bwd, x.device, C.byref(d), _p(dy), _p(x), _p(res), _p(dx), _p(dres), _p(stats), _p(gamma), _p(beta),
+            _p(dgamma), _p(dbeta), _p(ws), _nbytes(ws))
+
+
+def _linear_desc(x, w, act):
+    _need(x.dim() >= 1 and w.dim() == 2 and x.dtype in _DT, "x has to be [..., K] and w [N, K], in float32 or bfloat16")
+    N, K = w.shape
+    _like("w", w, "x", x, (N, x.shape[-1]))
+    _need(act in ACTS.values(), "activation %r", act)
+    d = LinearDesc()
+    m = 1
+    for n in x.shape[:-1]:
+        m *= n
+    d.dtype, d.M, d.N, d.K, d.act, d.dw_dtype = _DT[x.dtype], m, N, K, act, F32
+    d.x_ld, d.w_ld = _pitch("x", x), _pitch("w", w)
+    return d
+
+
+def linear_act_workspace(x, w, act=ACT_NONE, backward=False):
+    """Workspace (a uint8 tensor) for linear_act_fwd on these operands, with backward also for linear_act_bwd."""
+    d = _linear_desc(x, w, act)
+    return _bytes(int(lib.cvg_linear_act_workspace(C.byref(d), int(backward))), x.device)
+
+
+def linear_act_fwd(x, w, y, bias=None, res=None, pre=None, act=ACT_NONE, ws=None):
+    """y = act(x @ w.T + bias) + res; x [..., K], w [N, K], y / res / pre [..., N], bias f32 [N].  pre receives the
+    activation's argument for linear_act_bwd."""
+    d = _linear_desc(x, w, act)
+    out = tuple(x.shape[:-1]) + (d.N,)
+    for n, t in (("y", y), ("res", res), ("pre", pre)):
+        _like(n, t, "x", x, out)
+    _like("bias", bias, "x", x, (d.N,), torch.float32)
+    _dense("bias", bias)
+    d.y_ld, d.res_ld, d.pre_ld = _pitch("y", y), _pitch("res", res), _pitch("pre", pre)
+    ws = _scratch(ws, 0 if ws is not None else int(lib.cvg_linear_act_workspace(C.byref(d), 0)), x.device)
+    _launch(lib.cvg_linear_act_fwd, x.device, C.byref(d), _p(x), _p(w), _p(bias), _p(res), _p(y), _p(pre), _p(ws), _nbytes(ws))
+
+
+def linear_act_bwd(dy, x, w, pre=None, dx=None, dw=None, dbias=None, act=ACT_NONE, ws=None):
+    """Gradients of linear_act_fwd, each optional: dx like x, dw [N, K] (float32 or x's type), dbias f32 [N].  An
+    activation needs the pre of the forward call; the gradient of res is dy itself."""
+    d = _linear_desc(x, w, act)
+    out = tuple(x.shape[:-1]) + (d.N,)
+    _like("dy", dy, "x", x, out)
+    _like("pre", pre, "x", x, out)
+    _like("dx", dx, "x", x)
+    if dw is not None:
+        _need(dw.dtype in (torch.float32, x.dtype), "dw is %s", dw.dtype)
+        _like("dw", dw, "x", x, w.shape, dw.dtype)
+        d.dw_dtype = _DT[dw.dtype]
+    _like("dbias", dbias, "x", x, (d.N,), torch.float32)
+    _dense("dbias", dbias)
+    d.dy_ld, d.pre_ld, d.dx_ld, d.dw_ld = _pitch("dy", dy), _pitch("pre", pre), _pitch("dx", dx), _pitch("dw", dw)
+    ws = _scratch(ws, 0 if ws is not None else int(lib.cvg_linear_act_workspace(C.byref(d), 1)), x.device)
+    _launch(lib.cvg_linear_act_bwd, x.device, C.byref(d), _p(dy), _p(x), _p(w), _p(pre), _p(dx), _p(dw), _p(dbias), _p(ws),
+            _nbytes(ws))
+
+
+def distill_topk(logits, top_val, top_idx, loss, row_loss, dlogits=None, row_weight=None, temperature=1.0, grad_scale=1.0):
+    """Distillation loss against a teacher's top logits, and its gradient: logits [..., V], top_val f32 / top_idx int32
+    [..., top], row_loss / row_weight f32 [...], loss f32 scalar (one element); dlogits like logits (or logits itself)."""
+    _need(logits.dim() >= 1 and logits.dtype in _DT, "logits have to be [..., V] in float32 or bfloat16")
+    rows = tuple(logits.shape[:-1])
+    _need(top_val.dim() >= 1, "top_val has to be [..., top]")
+    d = DistillDesc()
+    d.dtype, d.V, d.top = _DT[logits.dtype], logits.shape[-1], top_val.shape[-1]
+    d.R = 1
+    for n in rows:
+        d.R *= n
+    _like("top_val", top_val, "logits", logits, rows + (d.top,), torch.float32)
+    _like("top_idx", top_idx, "logits", logits, rows + (d.top,), torch.int32)
+    _like("row_loss", row_loss, "logits", logits, rows, torch.float32)
+    _like("row_weight", row_weight, "logits", logits, rows, torch.float32)
+    _like("dlogits", dlogits, "logits", logits)
+    _need(loss.numel() == 1 and loss.dtype == torch.float32 and loss.device == logits.device, "loss has to be one float32 on %s",
+          logits.device)
+    _dense("row_loss", row_loss)
+    _dense("row_weight", row_weight)
+    d.logits_ld, d.dlogits_ld = _pitch("logits", logits), _pitch("dlogits", dlogits)
+    d.top_ld = _pitch("top_val", top_val)
+    _need((d.top_ld or d.top) == (_pitch("top_idx", top_idx) or d.top), "top_val and top_idx have to share their strides")
+    d.temperature, d.grad_scale = float(temperature), float(grad_scale)
+    _launch(lib.cvg_distill_topk, logits.device, C.byref(d), _p(logits), _p(top_val), _p(top_idx), _p(row_weight), _p(loss),
+            _p(row_loss), _p(dlogits))

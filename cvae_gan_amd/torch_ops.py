@@ -9,7 +9,8 @@ stream.  Two groups:
   ResNetEncoder.forward, ConvUpSampleDecoder.forward (models/networks.py:193-196, :159-162) and
   their autograd backward passes;
 * tensor-only operators that map one to one onto C entry points without a descriptor struct:
-  bn_stats, bn_act_fwd, bn_act_bwd, reparam_kl_fwd, mse_fwd_bwd, adamw.
+  bn_stats, bn_act_fwd, bn_act_bwd, reparam_kl_fwd, mse_fwd_bwd, adamw, gn_act_fwd, gn_act_bwd,
+  linear_act_fwd, linear_act_bwd, distill_topk (arguments as in cvae_gan_amd/ops.py; ws None: allocated).
 
 They are implemented for the CUDA dispatch key only (ROCm devices dispatch there); there is no
 CPU implementation, so a CPU tensor fails in the dispatcher instead of taking another path."""
@@ -57,6 +58,16 @@ _DEF.define("mse_fwd_bwd(Tensor dec, Tensor x, Tensor(a!) d_dec, Tensor(b!) ll, 
             "Tensor(c!) ws) -> ()")
 _DEF.define("adamw(Tensor(a!) p, Tensor g, Tensor(b!) m, Tensor(c!) v, float lr, float beta1, float beta2, float eps, "
             "float weight_decay, int step) -> ()")
+_DEF.define("gn_act_fwd(Tensor x, Tensor? res, Tensor(a!) y, int groups, Tensor(b!)? stats, Tensor gamma, Tensor beta, "
+            "float eps, int act, Tensor(c!)? ws) -> ()")
+_DEF.define("gn_act_bwd(Tensor dy, Tensor x, Tensor? res, Tensor(a!) dx, Tensor(b!)? dres, int groups, Tensor stats, Tensor gamma, "
+            "Tensor beta, Tensor(c!) dgamma, Tensor(d!) dbeta, int act, Tensor(e!)? ws) -> ()")
+_DEF.define("linear_act_fwd(Tensor x, Tensor w, Tensor(a!) y, Tensor? bias, Tensor? res, Tensor(b!)? pre, int act, "
+            "Tensor(c!)? ws) -> ()")
+_DEF.define("linear_act_bwd(Tensor dy, Tensor x, Tensor w, Tensor? pre, Tensor(a!)? dx, Tensor(b!)? dw, Tensor(c!)? dbias, int act, "
+            "Tensor(d!)? ws) -> ()")
+_DEF.define("distill_topk(Tensor logits, Tensor top_val, Tensor top_idx, Tensor(a!) loss, Tensor(b!) row_loss, "
+            "Tensor(c!)? dlogits, Tensor? row_weight, float temperature, float grad_scale) -> ()")
 
 _IMPL = Library("cvaegan", "IMPL", "CUDA")
 
@@ -115,11 +126,35 @@ def _adamw(p, g, m, v, lr, beta1, beta2, eps, weight_decay, step):
     ops.adamw(p, g, m, v, p.numel(), lr, beta1, beta2, eps, weight_decay, step)
 
 
+def _gn_act_fwd(x, res, y, groups, stats, gamma, beta, eps, act, ws):
+    ops.gn_act_fwd(x, res, y, groups, stats, gamma, beta, eps=eps, act=act, ws=ws)
+
+
+def _gn_act_bwd(dy, x, res, dx, dres, groups, stats, gamma, beta, dgamma, dbeta, act, ws):
+    ops.gn_act_bwd(dy, x, res, dx, dres, groups, stats, gamma, beta, dgamma, dbeta, act=act, ws=ws)
+
+
+def _linear_act_fwd(x, w, y, bias, res, pre, act, ws):
+    ops.linear_act_fwd(x, w, y, bias=bias, res=res, pre=pre, act=act, ws=ws)
+
+
+def _linear_act_bwd(dy, x, w, pre, dx, dw, dbias, act, ws):
+    ops.linear_act_bwd(dy, x, w, pre=pre, dx=dx, dw=dw, dbias=dbias, act=act, ws=ws)
+
+
+def _distill_topk(logits, top_val, top_idx, loss, row_loss, dlogits, row_weight, temperature, grad_scale):
+    ops.distill_topk(logits, top_val, top_idx, loss, row_loss, dlogits=dlogits, row_weight=row_weight, temperature=temperature,
+                     grad_scale=grad_scale)
+
+
 for _name, _fn in (("encoder_forward", _encoder_forward), ("encoder_backward", _encoder_backward),
                    ("decoder_forward", _decoder_forward), ("decoder_backward", _decoder_backward),
                    ("bn_stats", _bn_stats), ("bn_act_fwd", _bn_act_fwd), ("bn_act_bwd", _bn_act_bwd),
-                   ("reparam_kl_fwd", _reparam_kl_fwd), ("mse_fwd_bwd", _mse_fwd_bwd), ("adamw", _adamw)):
+                   ("reparam_kl_fwd", _reparam_kl_fwd), ("mse_fwd_bwd", _mse_fwd_bwd), ("adamw", _adamw),
+                   ("gn_act_fwd", _gn_act_fwd), ("gn_act_bwd", _gn_act_bwd), ("linear_act_fwd", _linear_act_fwd),
+                   ("linear_act_bwd", _linear_act_bwd), ("distill_topk", _distill_topk)):
     _IMPL.impl(_name, _fn)
 
 OPS = ["encoder_forward", "encoder_backward", "decoder_forward", "decoder_backward", "bn_stats", "bn_act_fwd",
-       "bn_act_bwd", "reparam_kl_fwd", "mse_fwd_bwd", "adamw"]
+       "bn_act_bwd", "reparam_kl_fwd", "mse_fwd_bwd", "adamw", "gn_act_fwd", "gn_act_bwd", "linear_act_fwd", "linear_act_bwd",
+       "distill_topk"]

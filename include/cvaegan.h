@@ -450,6 +450,75 @@ int cvg_gan_pair_feature_match(const void* h, int32_t dtype, int32_t ld, int32_t
  * gradients arriving from several critics).                                                     */
 int cvg_axpy_f32(float* y, const float* x, float alpha, int64_t n, cvg_stream s);
 
+/* ---- group normalisation, fused linear layers, distillation ------------------------------------------------
+ * Operators beside the reference's BatchNorm + LeakyReLU, Linear and loss calls (models/networks.py:173-191,
+ * models/cvae.py:137-139) for networks that normalise per sample, keep weights unpacked or learn from a teacher.
+ * None has a counterpart in the reference.  Workspaces need no initial contents and keep nothing between calls;
+ * calls whose kernels may overlap (other streams, other captured graphs) need workspaces of their own.
+ * Results do not depend on scheduling: every sum has a fixed order.                                          */
+enum { CVG_ACT_NONE = 0, CVG_ACT_LRELU = 1 /* slope 0.2 */, CVG_ACT_SILU = 2, CVG_ACT_GELU = 3 /* tanh form */ };
+
+/* Group normalisation with an activation, channels last:
+ *   y = act( gamma[c] * (x - mean) * rstd + beta[c] [+ res] ),  mean and rstd = 1 / sqrt(var + eps) (biased
+ * variance) over the HW pixels and C / G channels of one sample and group.
+ * Tensors are [B * HW] pixel rows of C channels at the pitches of the descriptor (elements, 0 = C).  C is a multiple
+ * of 8, G divides C, the least common multiple of 8 and C / G is at most 4096; pointers are 16-byte aligned and
+ * pitches multiples of 16 bytes.  B may be 0.
+ * stats f32 [2][B][G] = mean, rstd: written by the forward call, read by the backward call.
+ * y may be x or res itself; other overlaps of an output with an input are not supported.                     */
+typedef struct cvg_gn_desc {
+    int32_t dtype, B, HW, C, G, act;
+    int32_t x_ld, res_ld, y_ld;              /* forward: x, res, y; backward: x, res, dy                        */
+    int32_t dx_ld, dres_ld;
+    float eps;
+} cvg_gn_desc;
+size_t cvg_gn_act_workspace(const cvg_gn_desc* d, int32_t backward);
+int cvg_gn_act_fwd(const cvg_gn_desc* d, const void* x, const void* res, void* y, float* stats, const float* gamma,
+                   const float* beta, void* ws, size_t ws_bytes, cvg_stream s);
+/* g = dy * act'(pre), pre recomputed from x, stats and res (NULL as in the forward call);
+ *   dx = rstd * (gamma g - mean_group(gamma g) - xhat mean_group(gamma g xhat)),  dres = g (may be NULL),
+ *   dgamma[c] = sum g xhat, dbeta[c] = sum g over samples and pixels (f32, overwritten).
+ * dx or dres may be dy itself.                                                                                */
+int cvg_gn_act_bwd(const cvg_gn_desc* d, const void* dy, const void* x, const void* res, void* dx, void* dres,
+                   const float* stats, const float* gamma, const float* beta, float* dgamma, float* dbeta,
+                   void* ws, size_t ws_bytes, cvg_stream s);
+
+/* Linear layer with its epilogue:  pre = x w^T + bias,  y = act(pre) [+ res].
+ *   x [M][K], w [N][K] (the layout of nn.Linear, unpacked), y / res / pre [M][N] in d->dtype, bias f32 [N] or NULL;
+ *   pre (may be NULL) receives the rounded argument of the activation for the backward call.
+ * Row pitches in elements (0 = dense); any M >= 0, N, K >= 1 and any element-aligned pointer; rows of whole 16 bytes
+ * at 16-byte aligned addresses take the fast paths.  y may be res itself.
+ * Products are exact, sums f32; f32 data uses exact-f32 MFMA.                                                  */
+typedef struct cvg_linear_desc {
+    int32_t dtype, M, N, K, act;
+    int32_t dw_dtype;                        /* type of dw: CVG_F32 or the type of the data                     */
+    int32_t x_ld, w_ld, y_ld, res_ld, pre_ld, dy_ld, dx_ld, dw_ld;
+} cvg_linear_desc;
+size_t cvg_linear_act_workspace(const cvg_linear_desc* d, int32_t backward);
+int cvg_linear_act_fwd(const cvg_linear_desc* d, const void* x, const void* w, const float* bias, const void* res,
+                       void* y, void* pre, void* ws, size_t ws_bytes, cvg_stream s);
+/* dz = dy * act'(pre) (rounded to d->dtype: it feeds the matrix units; without an activation dz is dy),
+ *   dx = dz w, dw = dz^T x, dbias = column sums of dy * act'(pre) in f32; each may be NULL.  The gradient of res is dy. */
+int cvg_linear_act_bwd(const cvg_linear_desc* d, const void* dy, const void* x, const void* w, const void* pre,
+                       void* dx, void* dw, float* dbias, void* ws, size_t ws_bytes, cvg_stream s);
+
+/* Distillation from a teacher's top logits: row r of the student's logits [R][V] (dtype) learns the distribution that
+ * top_val [R][top] (f32, pitch top_ld) put on the classes top_idx [R][top] (int32, same pitch):
+ *   p = softmax(top_val / T) over the row's entries, q = softmax(logits / T) over all V classes,
+ *   row_loss[r] = row_weight[r] T^2 sum_j p_j (log p_j - log q[idx_j]),  *loss = sum_r row_loss[r],
+ *   dlogits[r][i] = grad_scale row_weight[r] T (q_i - sum of p_j with idx_j = i).
+ * An entry whose index lies outside [0, V) is absent (rows with fewer than `top` teacher entries); an index may
+ * appear twice.  A row of weight 0, or without an entry of finite value or NaN, has loss and gradient 0 whatever it
+ * holds.  row_weight f32 [R] or NULL (ones); row_loss f32 [R]; dlogits (dtype, pitch dlogits_ld) or NULL;
+ * dlogits may be logits itself.  R >= 0, 1 <= V, 1 <= top <= 1024, T > 0; pitches 0 = dense.                    */
+typedef struct cvg_distill_desc {
+    int32_t dtype, R, V, top;
+    int32_t logits_ld, dlogits_ld, top_ld;
+    float temperature, grad_scale;
+} cvg_distill_desc;
+int cvg_distill_topk(const cvg_distill_desc* d, const void* logits, const float* top_val, const int32_t* top_idx,
+                     const float* row_weight, float* loss, float* row_loss, void* dlogits, cvg_stream s);
+
 #ifdef __cplusplus
 }
 #endif

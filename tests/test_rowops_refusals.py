@@ -1,0 +1,164 @@
+"""What the group-norm, linear and distillation entry points refuse, without a GPU: every call here must fail in
+validation, before anything is launched (pointers are made-up aligned addresses that are never read)."""
+import ctypes as C
+
+import pytest
+import torch
+
+FAKE = 1 << 20
+
+
+def refused(fn, *args):
+    from cvae_gan_amd import _lib
+    rc = fn(*args)
+    assert rc != 0
+    return _lib.lib.cvg_last_error().decode()
+
+
+def gn(**kw):
+    from cvae_gan_amd._lib import GnDesc
+    d = GnDesc()
+    base = dict(dtype=1, B=2, HW=16, C=64, G=8, act=2, eps=1e-5)
+    base.update(kw)
+    for k, v in base.items():
+        setattr(d, k, v)
+    return d
+
+
+@pytest.mark.parametrize("kw, needle", [
+    (dict(dtype=2), "dtype"), (dict(C=12, G=4), "multiple of 8"), (dict(G=7), "divide"), (dict(HW=0), "HW"), (dict(B=-1), "B -1"),
+    (dict(act=4), "activation"), (dict(act=-1), "activation"), (dict(C=8192, G=1), "too wide"), (dict(C=8 * 1027, G=8), "too wide"),
+    (dict(x_ld=56), "pitch"), (dict(y_ld=68), "pitch"), (dict(dres_ld=-64), "pitch"), (dict(eps=-1.0), "eps"),
+    (dict(B=1 << 20, HW=1 << 12), "pixel rows"), (dict(G=0), "G 0"),
+])
+def test_group_norm_descriptors(kw, needle):
+    from cvae_gan_amd._lib import lib
+    d = C.byref(gn(**kw))
+    assert needle in refused(lib.cvg_gn_act_fwd, d, FAKE, None, FAKE, FAKE, FAKE, FAKE, FAKE, 1 << 30, None)
+    assert needle in refused(lib.cvg_gn_act_bwd, d, FAKE, FAKE, None, FAKE, None, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, 1 << 30, None)
+    assert lib.cvg_gn_act_workspace(d, 1) == 0
+
+
+def test_group_norm_pointers_and_workspaces():
+    from cvae_gan_amd._lib import lib
+    d = C.byref(gn(HW=1 << 20))
+    fwd, bwd = lib.cvg_gn_act_fwd, lib.cvg_gn_act_bwd
+    assert "null" in refused(fwd, d, None, None, FAKE, FAKE, FAKE, FAKE, FAKE, 1 << 40, None)
+    assert "null" in refused(fwd, d, FAKE, None, FAKE, FAKE, None, FAKE, FAKE, 1 << 40, None)
+    assert "16-byte" in refused(fwd, d, FAKE + 2, None, FAKE, FAKE, FAKE, FAKE, FAKE, 1 << 40, None)
+    assert "16-byte" in refused(fwd, d, FAKE, FAKE + 8, FAKE, FAKE, FAKE, FAKE, FAKE, 1 << 40, None)
+    assert lib.cvg_gn_act_workspace(d, 0) > 0
+    assert "workspace" in refused(fwd, d, FAKE, None, FAKE, FAKE, FAKE, FAKE, FAKE, lib.cvg_gn_act_workspace(d, 0) - 1, None)
+    assert "workspace" in refused(fwd, d, FAKE, None, FAKE, FAKE, FAKE, FAKE, None, 1 << 40, None)
+    assert "null" in refused(bwd, d, FAKE, FAKE, None, FAKE, None, None, FAKE, FAKE, FAKE, FAKE, FAKE, 1 << 40, None)
+    assert "null" in refused(bwd, d, FAKE, FAKE, None, FAKE, None, FAKE, FAKE, FAKE, None, FAKE, FAKE, 1 << 40, None)
+    assert "workspace" in refused(bwd, d, FAKE, FAKE, None, FAKE, None, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, 16, None)
+
+
+def lin(**kw):
+    from cvae_gan_amd._lib import LinearDesc
+    d = LinearDesc()
+    base = dict(dtype=1, M=4, N=32, K=16, act=2, dw_dtype=0)
+    base.update(kw)
+    for k, v in base.items():
+        setattr(d, k, v)
+    return d
+
+
+@pytest.mark.parametrize("kw, needle", [
+    (dict(dtype=3), "dtype"), (dict(dtype=0, dw_dtype=1), "dw_dtype"), (dict(M=-1), "M -1"), (dict(N=0), "N 0"), (dict(K=0), "K 0"),
+    (dict(act=9), "activation"), (dict(x_ld=15), "pitch"), (dict(w_ld=8), "pitch"), (dict(y_ld=31), "pitch"), (dict(dy_ld=-1), "pitch"),
+])
+def test_linear_descriptors(kw, needle):
+    from cvae_gan_amd._lib import lib
+    d = C.byref(lin(**kw))
+    assert needle in refused(lib.cvg_linear_act_fwd, d, FAKE, FAKE, None, None, FAKE, None, FAKE, 1 << 40, None)
+    assert needle in refused(lib.cvg_linear_act_bwd, d, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, 1 << 40, None)
+
+
+def test_linear_pointers_and_workspaces():
+    from cvae_gan_amd._lib import lib
+    d = C.byref(lin())
+    fwd, bwd = lib.cvg_linear_act_fwd, lib.cvg_linear_act_bwd
+    assert "null" in refused(fwd, d, FAKE, None, None, None, FAKE, None, FAKE, 1 << 40, None)
+    assert "misaligned" in refused(fwd, d, FAKE + 1, FAKE, None, None, FAKE, None, FAKE, 1 << 40, None)
+    assert "pre" in refused(bwd, d, FAKE, FAKE, FAKE, None, FAKE, None, None, FAKE, 1 << 40, None)
+    assert "needs w" in refused(bwd, d, FAKE, FAKE, None, FAKE, FAKE, None, None, FAKE, 1 << 40, None)
+    assert "needs x" in refused(bwd, d, FAKE, None, FAKE, FAKE, None, FAKE, None, FAKE, 1 << 40, None)
+    assert "misaligned dw" in refused(bwd, d, FAKE, FAKE, FAKE, FAKE, None, FAKE + 2, None, FAKE, 1 << 40, None)
+    assert "workspace" in refused(bwd, d, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, lib.cvg_linear_act_workspace(d, 1) - 1, None)
+    assert "workspace" in refused(bwd, d, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE + 4, 1 << 40, None)
+
+
+@pytest.mark.parametrize("kw, needle", [
+    (dict(dtype=5), "dtype"), (dict(V=0), "V 0"), (dict(R=-2), "R -2"), (dict(top=0), "teacher entries"), (dict(top=1025), "teacher entries"),
+    (dict(temperature=0.0), "temperature"), (dict(temperature=-1.0), "temperature"), (dict(temperature=float("nan")), "temperature"),
+    (dict(temperature=float("inf")), "temperature"), (dict(logits_ld=99), "pitches"), (dict(dlogits_ld=1), "pitches"),
+    (dict(top_ld=3), "pitches"),
+])
+def test_distill_descriptors(kw, needle):
+    from cvae_gan_amd._lib import lib, DistillDesc
+    d = DistillDesc()
+    base = dict(dtype=1, R=4, V=100, top=5, temperature=1.0, grad_scale=1.0)
+    base.update(kw)
+    for k, v in base.items():
+        setattr(d, k, v)
+    assert needle in refused(lib.cvg_distill_topk, C.byref(d), FAKE, FAKE, FAKE, None, FAKE, FAKE, FAKE, None)
+
+
+def test_distill_pointers():
+    from cvae_gan_amd._lib import lib, DistillDesc
+    d = DistillDesc()
+    d.dtype, d.R, d.V, d.top, d.temperature = 1, 4, 100, 5, 1.0
+    f = lib.cvg_distill_topk
+    assert "null loss" in refused(f, C.byref(d), FAKE, FAKE, FAKE, None, None, FAKE, FAKE, None)
+    assert "null tensor" in refused(f, C.byref(d), FAKE, None, FAKE, None, FAKE, FAKE, FAKE, None)
+    assert "misaligned" in refused(f, C.byref(d), FAKE + 1, FAKE, FAKE, None, FAKE, FAKE, None, None)
+    d.logits_ld = 128
+    assert "in place" in refused(f, C.byref(d), FAKE, FAKE, FAKE, None, FAKE, FAKE, FAKE, None)
+
+
+def bad(call, needle):
+    from cvae_gan_amd.ops import CvgError
+    with pytest.raises(CvgError, match=needle):
+        call()
+
+
+def test_tensor_checks():
+    """Shapes, types and strides are refused by the tensor layer; a CPU tensor is refused last."""
+    from cvae_gan_amd import ops
+    x, one = torch.zeros(2, 4, 4, 16), torch.ones(16)
+    st = torch.zeros(2, 2, 4)
+    y = torch.zeros_like(x)
+    bad(lambda: ops.gn_act_fwd(x, None, y, 4, st, one, one), "device tensors")
+    bad(lambda: ops.gn_act_fwd(x, None, y[:1], 4, st, one, one), "y has shape")
+    bad(lambda: ops.gn_act_fwd(x, None, y.bfloat16(), 4, st, one, one), "y is torch.bfloat16")
+    bad(lambda: ops.gn_act_fwd(x, None, y, 4, st, one[:8], one), "gamma has shape")
+    bad(lambda: ops.gn_act_fwd(x, None, y, 4, st.double(), one, one), "stats is")
+    bad(lambda: ops.gn_act_fwd(x, None, y, 2, st, one, one), "stats has shape")
+    bad(lambda: ops.gn_act_fwd(x.half(), None, y, 4, st, one, one), "bfloat16")
+    bad(lambda: ops.gn_act_fwd(x, None, y, 4, st, one, one, act=7), "activation")
+    bad(lambda: ops.gn_act_fwd(x.permute(0, 3, 1, 2), None, y.permute(0, 3, 1, 2), 4, st, torch.ones(4), torch.ones(4)), "consecutive")
+    bad(lambda: ops.gn_act_fwd(torch.zeros(2, 8, 4, 16)[:, ::2], None, y, 4, st, one, one), "one pitch")
+    bad(lambda: ops.gn_act_fwd(torch.zeros(1, 1, 1, 16).expand(2, 4, 4, 16), None, y, 4, st, one, one), "overlap")
+    bad(lambda: ops.gn_act_bwd(y, x, None, y, None, 4, st, one, one, one, one[:3]), "dbeta has shape")
+    xl, w, yl = torch.zeros(3, 5, 16), torch.zeros(8, 16), torch.zeros(3, 5, 8)
+    bad(lambda: ops.linear_act_fwd(xl, w, yl), "device tensors")
+    bad(lambda: ops.linear_act_fwd(xl, w[:, :8], yl), "w has shape")
+    bad(lambda: ops.linear_act_fwd(xl, w.bfloat16(), yl), "w is")
+    bad(lambda: ops.linear_act_fwd(xl, w, yl[..., :4]), "y has shape")
+    bad(lambda: ops.linear_act_fwd(xl, w.t().contiguous().t(), yl), "consecutive")
+    bad(lambda: ops.linear_act_fwd(xl, w, yl, bias=torch.zeros(8, dtype=torch.bfloat16)), "bias is")
+    bad(lambda: ops.linear_act_fwd(xl, w, yl, res=torch.zeros(3, 5, 1).expand(3, 5, 8)), "consecutive")
+    bad(lambda: ops.linear_act_bwd(yl, xl, w, dw=w.bfloat16()), "dw is")
+    bad(lambda: ops.linear_act_bwd(yl, xl, w, dx=xl[:2]), "dx has shape")
+    lg, tv, ti = torch.zeros(4, 50), torch.zeros(4, 3), torch.zeros(4, 3, dtype=torch.int32)
+    loss, rl = torch.zeros(()), torch.zeros(4)
+    bad(lambda: ops.distill_topk(lg, tv, ti, loss, rl), "device tensors")
+    bad(lambda: ops.distill_topk(lg, tv, ti.long(), loss, rl), "top_idx is")
+    bad(lambda: ops.distill_topk(lg, tv, ti[:, :2], loss, rl), "top_idx has shape")
+    bad(lambda: ops.distill_topk(lg, tv, ti, torch.zeros(2), rl), "loss has to be")
+    bad(lambda: ops.distill_topk(lg, tv, ti, loss, rl[:3]), "row_loss has shape")
+    bad(lambda: ops.distill_topk(lg, tv.bfloat16(), ti, loss, rl), "top_val is")
+    bad(lambda: ops.distill_topk(lg, tv, torch.zeros(4, 5, dtype=torch.int32)[:, :3], loss, rl), "share their strides")
+    bad(lambda: ops.distill_topk(lg, tv, ti, loss, rl, dlogits=lg[:, :49]), "dlogits has shape")
