@@ -47,7 +47,7 @@ class GnDesc(C.Structure):
 
 
 class LinearDesc(C.Structure):
-    _fields_ = [(n, C.c_int32) for n in ("dtype", "M", "N", "K", "act", "dw_dtype", "x_ld", "w_ld", "y_ld", "res_ld", "pre_ld",
+    _fields_ = [(n, C.c_int32) for n in ("dtype", "M", "N", "K", "act", "dw_dtype", "pre_dtype", "x_ld", "w_ld", "y_ld", "res_ld", "pre_ld",
                                          "dy_ld", "dx_ld", "dw_ld")]
 
 

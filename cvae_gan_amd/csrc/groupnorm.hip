@@ -191,10 +191,10 @@ __global__ void __launch_bounds__(1024) gn_fwd_tile(const GnArgs a) {
             if (a.res) load8<T>(rp + (size_t)r * a.res_ld, q);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                float u = (v[j] - mean[j]) * sc[j] + be[j];
-                if (a.res) u += q[j];
-                v[j] = act_value<EXACT>(u, a.act);
+                v[j] = (v[j] - mean[j]) * sc[j] + be[j];
+                if (a.res) v[j] += q[j];
             }
+            act_value8<EXACT>(v, a.act);
             store8<T>(yp + (size_t)r * a.y_ld, v);
         }
     }
@@ -246,10 +246,10 @@ __global__ void __launch_bounds__(512) gn_fwd_apply(const GnArgs a) {
         if (a.res) load8<T>((const T*)a.res + (row0 + r) * a.res_ld + c, q);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            float u = (v[j] - mean[j]) * sc[j] + be[j];
-            if (a.res) u += q[j];
-            v[j] = act_value<EXACT>(u, a.act);
+            v[j] = (v[j] - mean[j]) * sc[j] + be[j];
+            if (a.res) v[j] += q[j];
         }
+        act_value8<EXACT>(v, a.act);
         store8<T>((T*)a.y + (row0 + r) * a.y_ld + c, v);
     }
 }
@@ -261,7 +261,7 @@ __device__ __forceinline__ void bwd_row(const Raw8<T>& xr, const Raw8<T>& dr, co
                                         const float (&mean)[8], const float (&rstd)[8], const float (&ga)[8], const float (&be)[8],
                                         float (&xh)[8], float (&g)[8]) {
     constexpr bool EXACT = sizeof(T) == 4;
-    float q[8];
+    float q[8], u[8];
     raw_f32(xr, xh);
     raw_f32(dr, g);
     if (has_res) raw_f32(rr, q);
@@ -269,10 +269,14 @@ __device__ __forceinline__ void bwd_row(const Raw8<T>& xr, const Raw8<T>& dr, co
     for (int j = 0; j < 8; ++j) {
         // the same expression as the forward pass, so that the sign LeakyReLU takes is the same
         const float d = xh[j] - mean[j];
-        float u = d * (ga[j] * rstd[j]) + be[j];
-        if (has_res) u += q[j];
+        u[j] = d * (ga[j] * rstd[j]) + be[j];
+        if (has_res) u[j] += q[j];
         xh[j] = d * rstd[j];
-        if (act != CVG_ACT_NONE) g[j] *= act_slope<EXACT>(u, act);
+    }
+    if (act != CVG_ACT_NONE) {
+        act_slope8<EXACT>(u, act);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) g[j] *= u[j];
     }
 }
 

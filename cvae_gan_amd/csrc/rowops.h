@@ -37,6 +37,26 @@ template <bool EXACT> __device__ __forceinline__ float act_slope(float v, int ac
         default: return 1.f;
     }
 }
+// eight values at once: the activation is chosen once, outside the loop
+template <bool EXACT, int ACT> __device__ __forceinline__ void act_value8_(float (&v)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = act_value<EXACT>(v[j], ACT);
+}
+template <bool EXACT, int ACT> __device__ __forceinline__ void act_slope8_(float (&v)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = act_slope<EXACT>(v[j], ACT);
+}
+template <bool EXACT> __device__ __forceinline__ void act_value8(float (&v)[8], int act) {
+    if (act == CVG_ACT_LRELU) act_value8_<EXACT, CVG_ACT_LRELU>(v);
+    else if (act == CVG_ACT_SILU) act_value8_<EXACT, CVG_ACT_SILU>(v);
+    else if (act == CVG_ACT_GELU) act_value8_<EXACT, CVG_ACT_GELU>(v);
+}
+template <bool EXACT> __device__ __forceinline__ void act_slope8(float (&v)[8], int act) {
+    if (act == CVG_ACT_LRELU) act_slope8_<EXACT, CVG_ACT_LRELU>(v);
+    else if (act == CVG_ACT_SILU) act_slope8_<EXACT, CVG_ACT_SILU>(v);
+    else if (act == CVG_ACT_GELU) act_slope8_<EXACT, CVG_ACT_GELU>(v);
+    else act_slope8_<EXACT, CVG_ACT_NONE>(v);
+}
 static inline bool act_known(int act) { return act >= CVG_ACT_NONE && act <= CVG_ACT_GELU; }
 
 __device__ __forceinline__ float wave_max(float v) {

@@ -462,9 +462,16 @@ def _linear_desc(x, w, act):
     m = 1
     for n in x.shape[:-1]:
         m *= n
-    d.dtype, d.M, d.N, d.K, d.act, d.dw_dtype = _DT[x.dtype], m, N, K, act, F32
+    d.dtype, d.M, d.N, d.K, d.act, d.dw_dtype, d.pre_dtype = _DT[x.dtype], m, N, K, act, F32, F32
     d.x_ld, d.w_ld = _pitch("x", x), _pitch("w", w)
     return d
+
+
+def _pre(d, pre, x, shape):
+    if pre is not None:
+        _need(pre.dtype in (torch.float32, x.dtype), "pre is %s", pre.dtype)
+        _like("pre", pre, "x", x, shape, pre.dtype)
+        d.pre_dtype = _DT[pre.dtype]
 
 
 def linear_act_workspace(x, w, act=ACT_NONE, backward=False):
@@ -474,12 +481,13 @@ def linear_act_workspace(x, w, act=ACT_NONE, backward=False):
 
 
 def linear_act_fwd(x, w, y, bias=None, res=None, pre=None, act=ACT_NONE, ws=None):
-    """y = act(x @ w.T + bias) + res; x [..., K], w [N, K], y / res / pre [..., N], bias f32 [N].  pre receives the
-    activation's argument for linear_act_bwd."""
+    """y = act(x @ w.T + bias) + res; x [..., K], w [N, K], y / res / pre [..., N], bias f32 [N].  pre (float32
+    or x's type) receives the activation's argument for linear_act_bwd."""
     d = _linear_desc(x, w, act)
     out = tuple(x.shape[:-1]) + (d.N,)
-    for n, t in (("y", y), ("res", res), ("pre", pre)):
+    for n, t in (("y", y), ("res", res)):
         _like(n, t, "x", x, out)
+    _pre(d, pre, x, out)
     _like("bias", bias, "x", x, (d.N,), torch.float32)
     _dense("bias", bias)
     d.y_ld, d.res_ld, d.pre_ld = _pitch("y", y), _pitch("res", res), _pitch("pre", pre)
@@ -493,7 +501,7 @@ def linear_act_bwd(dy, x, w, pre=None, dx=None, dw=None, dbias=None, act=ACT_NON
     d = _linear_desc(x, w, act)
     out = tuple(x.shape[:-1]) + (d.N,)
     _like("dy", dy, "x", x, out)
-    _like("pre", pre, "x", x, out)
+    _pre(d, pre, x, out)
     _like("dx", dx, "x", x)
     if dw is not None:
         _need(dw.dtype in (torch.float32, x.dtype), "dw is %s", dw.dtype)

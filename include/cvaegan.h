@@ -485,13 +485,14 @@ int cvg_gn_act_bwd(const cvg_gn_desc* d, const void* dy, const void* x, const vo
 
 /* Linear layer with its epilogue:  pre = x w^T + bias,  y = act(pre) [+ res].
  *   x [M][K], w [N][K] (the layout of nn.Linear, unpacked), y / res / pre [M][N] in d->dtype, bias f32 [N] or NULL;
- *   pre (may be NULL) receives the rounded argument of the activation for the backward call.
- * Row pitches in elements (0 = dense); any M >= 0, N, K >= 1 and any element-aligned pointer; rows of whole 16 bytes
+ *   pre (may be NULL) receives the argument of the activation for the backward call, in d->pre_dtype: f32 keeps its
+ *   derivative, and with it dbias, at f32 accuracy; the type of the data halves what the backward call reads.
+ * Row pitches in elements (0 = dense); any M >= 0, N and K from 1 to 2000000, and any element-aligned pointer; rows of whole 16 bytes
  * at 16-byte aligned addresses take the fast paths.  y may be res itself.
  * Products are exact, sums f32; f32 data uses exact-f32 MFMA.                                                  */
 typedef struct cvg_linear_desc {
     int32_t dtype, M, N, K, act;
-    int32_t dw_dtype;                        /* type of dw: CVG_F32 or the type of the data                     */
+    int32_t dw_dtype, pre_dtype;             /* types of dw and pre: CVG_F32 or the type of the data            */
     int32_t x_ld, w_ld, y_ld, res_ld, pre_ld, dy_ld, dx_ld, dw_ld;
 } cvg_linear_desc;
 size_t cvg_linear_act_workspace(const cvg_linear_desc* d, int32_t backward);

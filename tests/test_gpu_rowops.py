@@ -210,16 +210,16 @@ LIN_CASES = [
     # M, N, K
     (1, 1, 1), (1, 64, 64), (1, 1000, 515), (2, 24, 8), (3, 136, 72), (16, 256, 512), (17, 100, 33), (33, 48, 200),
     (64, 512, 128), (100, 77, 129), (130, 264, 264), (256, 128, 1096), (300, 520, 96), (515, 9, 17), (777, 303, 115), (513, 512, 320),
-    (1, 4096, 1032), (5, 2056, 24), (48, 640, 1024), (2048, 40, 8),
+    (1, 4096, 1032), (5, 2056, 24), (48, 640, 1024), (2048, 40, 8), (1030, 776, 200),
 ]
 
 
-def lin_check(ops, x, w, bias, res, dy, act, dw_dtype, what, ws=None):
+def lin_check(ops, x, w, bias, res, dy, act, dw_dtype, what, ws=None, pre_dtype=None):
     M, N, K = x.shape[0], w.shape[0], w.shape[1]
     dtype = x.dtype
     nan = float("nan")
     y = torch.full((M, N), nan, dtype=dtype, device="cuda")
-    pre = torch.full((M, N), nan, dtype=dtype, device="cuda")
+    pre = torch.full((M, N), nan, dtype=pre_dtype or dtype, device="cuda")
     a = ops.ACTS[act]
     ops.linear_act_fwd(x, w, y, bias=bias, res=res, pre=pre, act=a, ws=ws)
     xd, wd = x.double(), w.double()
@@ -253,7 +253,7 @@ def test_linear(ops, case, dtype):
     bias, dy, res = rnd(g, N), rnd(g, M, N, dtype=dtype), rnd(g, M, N, dtype=dtype)
     lin_check(ops, x, w, bias, None, dy, "none", F32, "none")
     lin_check(ops, x, w, bias, res, dy, "gelu", dtype, "gelu")
-    lin_check(ops, x, w, None, None, dy, "silu", F32, "silu")
+    lin_check(ops, x, w, None, None, dy, "silu", F32, "silu", pre_dtype=F32)
     lin_check(ops, x, w, None, res, dy, "lrelu", dtype, "lrelu")
 
 

@@ -76,6 +76,21 @@ def test_linear_descriptors(kw, needle):
     assert needle in refused(lib.cvg_linear_act_bwd, d, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, 1 << 40, None)
 
 
+def test_linear_workspace_sizes():
+    """Plans over ordinary and degenerate sizes: no division by an empty range, sizes bounded by the operands'."""
+    from cvae_gan_amd._lib import lib
+    for dtype in (0, 1):
+        for M in (0, 1, 7, 64, 1000, 100000):
+            for N in (1, 64, 1003, 2000000):
+                for K in (1, 8, 515, 8192):
+                    d = C.byref(lin(dtype=dtype, M=M, N=N, K=K))
+                    f, b = lib.cvg_linear_act_workspace(d, 0), lib.cvg_linear_act_workspace(d, 1)
+                    if lib.cvg_linear_act_fwd(d, None, None, None, None, None, None, None, 0, None) != 0 and f == 0:
+                        assert b"too many" in lib.cvg_last_error()
+                        continue
+                    assert 0 < f <= b < 1 << 50
+
+
 def test_linear_pointers_and_workspaces():
     from cvae_gan_amd._lib import lib
     d = C.byref(lin())
