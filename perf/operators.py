@@ -166,7 +166,8 @@ def _buffers(s):
         x, w = s["x"], s["w"]
         s["act"] = ops.ACTS[c["act"]]
         s["y"] = torch.empty(c["rows"], c["n"], dtype=x.dtype, device=x.device)
-        s["pre"] = torch.empty_like(s["y"]) if c["train"] and c["act"] != "none" else None
+        # f32: the bias gradient, an f32 sum, keeps the digits of the activation's derivative
+        s["pre"] = torch.empty_like(s["y"], dtype=torch.float32) if c["train"] and c["act"] != "none" else None
         s["ws"] = ops.linear_act_workspace(x, w, act=s["act"], backward=c["train"])
         if c["train"]:
             s["dx"] = torch.empty_like(x)
