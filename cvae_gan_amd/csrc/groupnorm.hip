@@ -20,6 +20,7 @@ struct GnArgs {
     int B, HW, C, G, act, tiles, rows_tile, nslab, nv, rpp, ent;
     int x_ld, res_ld, y_ld, dx_ld, dres_ld;
     float eps;
+    int seg;                         // lanes that sum one group (a power of two)
     FastDiv cg, nvd, tiled, slabd;   // divisions by C / G, nv, tiles, nslab
 };
 
@@ -33,10 +34,27 @@ struct Place {
 __device__ __forceinline__ Place gn_place(const GnArgs& a) {
     Place p;
     uint32_t blk = blockIdx.x;
-    const uint32_t bs = fdiv(blk, a.tiled);
-    p.tile = blk - bs * a.tiles;
-    p.b = fdiv(bs, a.slabd);
-    const int slab = bs - p.b * a.nslab;
+    uint32_t slab;
+    if (a.tiles == 1) {
+        // Workgroups go round-robin over the 8 dies: the slabs of one sample are given to one die, one after the other,
+        // because a slab may be narrower than the 128-byte lines they share.
+        const uint32_t q = blk >> 3, whole = (uint32_t)(a.B & ~7) * a.nslab;
+        p.tile = 0;
+        if (blk < whole) {
+            const uint32_t grp = fdiv(q, a.slabd);
+            slab = q - grp * a.nslab;
+            p.b = grp * 8 + (blk & 7);
+        } else {
+            const uint32_t rest = blk - whole, bb = fdiv(rest, a.slabd);
+            slab = rest - bb * a.nslab;
+            p.b = (a.B & ~7) + bb;
+        }
+    } else {
+        const uint32_t bs = fdiv(blk, a.tiled);
+        p.tile = blk - bs * a.tiles;
+        p.b = fdiv(bs, a.slabd);
+        slab = bs - p.b * a.nslab;
+    }
     p.c0 = slab * a.nv * 8;
     p.nch = min(a.nv * 8, a.C - p.c0);
     p.nv = p.nch >> 3;
@@ -50,59 +68,90 @@ __device__ __forceinline__ Place gn_place(const GnArgs& a) {
     return p;
 }
 
-// Column sums over the workgroup: N values per channel of the slab, sm[n][ent][nv * 8]; afterwards sm[n][0][c] holds
-// the sum of channel c.  Where the chunk count is a power of two up to 32 the lanes of a wave that hold the same chunk
-// are added by shuffles first, which leaves one entry per wave, otherwise one per row lane.
+// Partial column sums: N values per channel of the slab into sm[n][ent][nv * 8], one entry per wave where a wave's lanes
+// share chunk columns evenly (a power of two up to 32 of them), otherwise one per row lane.  Up to 8 chunk columns the
+// lanes split the eight channels among themselves while they add (4 + 2 + 1 shuffles, then one for each remaining
+// halving) instead of carrying all eight through every step.
 template <int N>
-__device__ __forceinline__ void column_sums(const GnArgs& a, const Place& p, float (&v)[N][8], float* sm) {
-    const int width = a.nv * 8;
+__device__ __forceinline__ void column_parts(const GnArgs& a, const Place& p, float (&v)[N][8], float* sm) {
+    const int width = a.nv * 8, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const bool fold = (a.nv & (a.nv - 1)) == 0 && a.nv <= 32;
-    int e = p.ty;
-    bool writes = p.ty < a.rpp;
-    if (fold) {
-        for (int o = a.nv; o < 64; o <<= 1)
+    if (fold && a.nv <= 8) {
+        const bool h32 = lane & 32, h16 = lane & 16, h8 = lane & 8;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[n][j] = (h32 ? v[n][j + 4] : v[n][j]) + __shfl_xor(h32 ? v[n][j] : v[n][j + 4], 32, 64);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) v[n][j] = (h16 ? v[n][j + 2] : v[n][j]) + __shfl_xor(h16 ? v[n][j] : v[n][j + 2], 16, 64);
+            v[n][0] = (h8 ? v[n][1] : v[n][0]) + __shfl_xor(h8 ? v[n][0] : v[n][1], 8, 64);
+        }
+        for (int o = a.nv; o < 8; o <<= 1)
+#pragma unroll
+            for (int n = 0; n < N; ++n) v[n][0] += __shfl_xor(v[n][0], o, 64);
+        __syncthreads();             // the last readers of sm are done
+        if ((lane & 7) < a.nv)
+#pragma unroll
+            for (int n = 0; n < N; ++n) sm[(n * a.ent + wave) * width + (lane & 7) * 8 + (h32 ? 4 : 0) + (h16 ? 2 : 0) + (h8 ? 1 : 0)] = v[n][0];
+    } else {
+        int e = p.ty;
+        bool writes = p.ty < a.rpp;
+        if (fold) {
+            for (int o = a.nv; o < 64; o <<= 1)
+#pragma unroll
+                for (int n = 0; n < N; ++n)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[n][j] += __shfl_xor(v[n][j], o, 64);
+            e = wave;
+            writes = lane < a.nv;
+        }
+        __syncthreads();
+        if (writes)
 #pragma unroll
             for (int n = 0; n < N; ++n)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[n][j] += __shfl_xor(v[n][j], o, 64);
-        e = threadIdx.x >> 6;
-        writes = (int)(threadIdx.x & 63) < a.nv;
+                for (int j = 0; j < 8; j += 4)
+                    *(f32x4*)&sm[(n * a.ent + e) * width + p.chunk * 8 + j] = f32x4{v[n][j], v[n][j + 1], v[n][j + 2], v[n][j + 3]};
     }
-    __syncthreads();                 // the last readers of sm are done
-    if (writes)
-#pragma unroll
-        for (int n = 0; n < N; ++n)
-#pragma unroll
-            for (int j = 0; j < 8; j += 4)
-                *(f32x4*)&sm[(n * a.ent + e) * width + p.chunk * 8 + j] = f32x4{v[n][j], v[n][j + 1], v[n][j + 2], v[n][j + 3]};
     __syncthreads();
+}
+// adds the entries: afterwards sm[n][0][c] holds the sum of channel c
+template <int N>
+__device__ __forceinline__ void column_totals(const GnArgs& a, float* sm) {
+    const int width = a.nv * 8;
     for (int t = threadIdx.x; t < N * width; t += blockDim.x) {
         const int n = t >= width ? 1 : 0, c = t - n * width;
         float* q = sm + (size_t)n * a.ent * width + c;
         float s = 0.f;
+#pragma unroll 8
         for (int i = 0; i < a.ent; ++i) s += q[i * width];
         q[0] = s;                    // only this thread touches column c
     }
     __syncthreads();
 }
 
-// sums[n][g] = sum over the channels of group g of w[c] * sm[n][0][c] (w = 1 where null): a wave per group, lanes over channels
+// sums[n][g] = sum over the channels of group g and the first `ent` entries of w[c] * sm[n][entry][c] (w = 1 where null):
+// a.seg lanes per group
 template <int N>
-__device__ __forceinline__ void group_sums(const GnArgs& a, const Place& p, const float* sm, const float* w, float (*sums)[GN_MAX_GROUPS]) {
-    const int cg = a.cg.d, width = a.nv * 8, lane = threadIdx.x & 63;
-    for (int g = threadIdx.x >> 6; g < p.ngr; g += blockDim.x >> 6) {
+__device__ __forceinline__ void group_sums(const GnArgs& a, const Place& p, const float* sm, const float* w, int ent, float (*sums)[GN_MAX_GROUPS]) {
+    const int cg = a.cg.d, width = a.nv * 8, lane = threadIdx.x & 63, seg = a.seg, per = 64 / seg;
+    const int n_items = ent * cg;
+    for (int base = (threadIdx.x >> 6) * per; base < p.ngr; base += (blockDim.x >> 6) * per) {
+        const int g = base + lane / seg;
         float s[N];
 #pragma unroll
         for (int n = 0; n < N; ++n) s[n] = 0.f;
-        for (int c = g * cg + lane; c < (g + 1) * cg; c += 64) {
-            const float k = w ? w[p.c0 + c] : 1.f;
+        if (g < p.ngr)
+            for (int i = lane & (seg - 1); i < n_items; i += seg) {
+                const int e = fdiv(i, a.cg), c = g * cg + i - e * cg;
+                const float k = w ? w[p.c0 + c] : 1.f;
 #pragma unroll
-            for (int n = 0; n < N; ++n) s[n] += k * sm[(size_t)n * a.ent * width + c];
-        }
+                for (int n = 0; n < N; ++n) s[n] += k * sm[(n * a.ent + e) * width + c];
+            }
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const float t = wave_sum(s[n]);
-            if (lane == 0) sums[n][g] = t;
+            for (int o = seg >> 1; o > 0; o >>= 1) s[n] += __shfl_xor(s[n], o, 64);
+            if (g < p.ngr && (lane & (seg - 1)) == 0) sums[n][g] = s[n];
         }
     }
     __syncthreads();
@@ -114,51 +163,69 @@ __device__ __forceinline__ void chunk_groups(const GnArgs& a, const Place& p, in
     for (int j = 0; j < 8; ++j) gi[j] = p.live ? fdiv(p.chunk * 8 + j, a.cg) : 0;
 }
 
-template <typename T, int R>
-__global__ void __launch_bounds__(1024) gn_fwd_tile(const GnArgs a) {
+// (keeps the unpacking of a row where it is written: hoisted, it would wait for every row at once)
+__device__ __forceinline__ void pin(Raw8<bf16>& r) { asm volatile("" : "+v"(r.a)); }
+__device__ __forceinline__ void pin(Raw8<float>& r) { asm volatile("" : "+v"(r.a), "+v"(r.b)); }
+
+// pre = x (gamma rstd) + (beta - mean gamma rstd) (+ res) in both passes, one fma: LeakyReLU takes the same sign twice.
+// Folding the mean into the constant costs an error of u |mean| gamma rstd, what the rounding of the mean itself costs.
+template <typename T, int ACT>
+__device__ __forceinline__ void apply_row(float (&v)[8], const float (&sc)[8], const float (&sh)[8], const float* q) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        v[j] = fmaf(v[j], sc[j], sh[j]);
+        if (q) v[j] += q[j];
+        v[j] = act_value<sizeof(T) == 4>(v[j], ACT);
+    }
+}
+
+template <typename T, int ACT, int R, int MAXT, int WAVES>
+__global__ void __launch_bounds__(MAXT, WAVES) gn_fwd_tile(const GnArgs a) {
     extern __shared__ float sm[];
     __shared__ float sums[2][GN_MAX_GROUPS];
-    constexpr bool EXACT = sizeof(T) == 4;
     const Place p = gn_place(a);
     const size_t row0 = (size_t)p.b * a.HW + p.r0;
-    const int rows = p.r1 - p.r0, c = p.c0 + p.chunk * 8;
+    const int rows = p.r1 - p.r0, c = p.c0 + (p.live ? p.chunk * 8 : 0);
+    float ga[8], be[8];                              // before the tile: what they wait for is short
+    load8<float>(a.gamma + c, ga);
+    load8<float>(a.beta + c, be);
     const T* xp = (const T*)a.x + row0 * a.x_ld + c;
     Raw8<T> xv[R];
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-        const int r = p.ty + i * a.rpp;
-        raw_zero(xv[i]);
-        if (p.live && r < rows) raw_load(xv[i], xp + (size_t)r * a.x_ld);
-    }
+    for (int i = 0; i < R; ++i) raw_load(xv[i], xp + (size_t)min(p.ty + i * a.rpp, rows - 1) * a.x_ld);
     int gi[8];
     chunk_groups(a, p, gi);
-    float acc[1][8];
+    const int mine = p.live ? rows : 0;              // rows this thread may count
+    float acc[1][8], mean[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) acc[0][j] = 0.f;
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-        float v[8];
-        raw_f32(xv[i], v);
+        if (p.ty + i * a.rpp < mine) {
+            float v[8];
+            pin(xv[i]);
+            raw_f32(xv[i], v);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) acc[0][j] += v[j];
+            for (int j = 0; j < 8; ++j) acc[0][j] += v[j];
+        }
     }
-    column_sums<1>(a, p, acc, sm);
-    group_sums<1>(a, p, sm, nullptr, sums);
+    column_parts<1>(a, p, acc, sm);
+    group_sums<1>(a, p, sm, nullptr, a.ent, sums);
     const float inv_n = 1.f / ((float)rows * (float)a.cg.d);
-    float mean[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) { mean[j] = sums[0][gi[j]] * inv_n; acc[0][j] = 0.f; }
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-        if (p.ty + i * a.rpp < rows && p.live) {
+        if (p.ty + i * a.rpp < mine) {
             float v[8];
+            pin(xv[i]);
             raw_f32(xv[i], v);
 #pragma unroll
             for (int j = 0; j < 8; ++j) { const float d = v[j] - mean[j]; acc[0][j] += d * d; }
         }
     }
-    column_sums<1>(a, p, acc, sm);
-    group_sums<1>(a, p, sm, nullptr, sums + 1);
+    column_parts<1>(a, p, acc, sm);
+    group_sums<1>(a, p, sm, nullptr, a.ent, sums + 1);
     if (a.tiles > 1) {
         for (int g = threadIdx.x; g < p.ngr; g += blockDim.x) {
             float* o = a.part + (((size_t)p.b * a.G + p.g0 + g) * a.tiles + p.tile) * 2;
@@ -173,37 +240,31 @@ __global__ void __launch_bounds__(1024) gn_fwd_tile(const GnArgs a) {
             a.stats[o] = sums[0][g] * inv_n;
             a.stats[(size_t)a.B * a.G + o] = 1.f / sqrtf(sums[1][g] * inv_n + a.eps);
         }
-    if (!p.live) return;
-    float sc[8], be[8];
+    float sc[8], sh[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        sc[j] = a.gamma[c + j] * (1.f / sqrtf(sums[1][gi[j]] * inv_n + a.eps));
-        be[j] = a.beta[c + j];
+        sc[j] = ga[j] * (1.f / sqrtf(sums[1][gi[j]] * inv_n + a.eps));
+        sh[j] = fmaf(-mean[j], sc[j], be[j]);
     }
     const T* rp = (const T*)a.res + row0 * a.res_ld + c;
     T* yp = (T*)a.y + row0 * a.y_ld + c;
 #pragma unroll
     for (int i = 0; i < R; ++i) {
         const int r = p.ty + i * a.rpp;
-        if (r < rows) {
+        if (r < mine) {
             float v[8], q[8];
-            raw_f32(xv[i], v);
             if (a.res) load8<T>(rp + (size_t)r * a.res_ld, q);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                v[j] = (v[j] - mean[j]) * sc[j] + be[j];
-                if (a.res) v[j] += q[j];
-            }
-            act_value8<EXACT>(v, a.act);
+            pin(xv[i]);
+            raw_f32(xv[i], v);
+            if (a.res) apply_row<T, ACT>(v, sc, sh, q); else apply_row<T, ACT>(v, sc, sh, nullptr);
             store8<T>(yp + (size_t)r * a.y_ld, v);
         }
     }
 }
 
 // Second kernel of the tiled form: every workgroup merges its sample's (mean, M2) partials, then applies.
-template <typename T>
-__global__ void __launch_bounds__(512) gn_fwd_apply(const GnArgs a) {
-    constexpr bool EXACT = sizeof(T) == 4;
+template <typename T, int ACT>
+__global__ void __launch_bounds__(1024) gn_fwd_apply(const GnArgs a) {
     __shared__ float mu[GN_MAX_GROUPS], rs[GN_MAX_GROUPS];
     const Place p = gn_place(a);
     const int lane = threadIdx.x & 63, cg = a.cg.d;
@@ -236,92 +297,101 @@ __global__ void __launch_bounds__(512) gn_fwd_apply(const GnArgs a) {
     int gi[8];
     chunk_groups(a, p, gi);
     const int c = p.c0 + p.chunk * 8;
-    float mean[8], sc[8], be[8];
+    float sc[8], sh[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) { mean[j] = mu[gi[j]]; sc[j] = a.gamma[c + j] * rs[gi[j]]; be[j] = a.beta[c + j]; }
+    for (int j = 0; j < 8; ++j) { sc[j] = a.gamma[c + j] * rs[gi[j]]; sh[j] = fmaf(-mu[gi[j]], sc[j], a.beta[c + j]); }
     const size_t row0 = (size_t)p.b * a.HW;
-    for (int r = p.r0 + p.ty; r < p.r1; r += a.rpp) {
-        float v[8], q[8];
-        load8<T>((const T*)a.x + (row0 + r) * a.x_ld + c, v);
-        if (a.res) load8<T>((const T*)a.res + (row0 + r) * a.res_ld + c, q);
+    constexpr int U = 4;                             // rows in flight per thread
+    for (int r0 = p.r0 + p.ty; r0 < p.r1; r0 += U * a.rpp) {
+        Raw8<T> xr[U], rr[U];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            v[j] = (v[j] - mean[j]) * sc[j] + be[j];
-            if (a.res) v[j] += q[j];
+        for (int u = 0; u < U; ++u) {
+            const int r = min(r0 + u * a.rpp, p.r1 - 1);
+            raw_load(xr[u], (const T*)a.x + (row0 + r) * a.x_ld + c);
+            if (a.res) raw_load(rr[u], (const T*)a.res + (row0 + r) * a.res_ld + c);
         }
-        act_value8<EXACT>(v, a.act);
-        store8<T>((T*)a.y + (row0 + r) * a.y_ld + c, v);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int r = r0 + u * a.rpp;
+            if (r < p.r1) {
+                float v[8], q[8];
+                raw_f32(xr[u], v);
+                if (a.res) raw_f32(rr[u], q);
+                if (a.res) apply_row<T, ACT>(v, sc, sh, q); else apply_row<T, ACT>(v, sc, sh, nullptr);
+                store8<T>((T*)a.y + (row0 + r) * a.y_ld + c, v);
+            }
+        }
     }
 }
 
 // ---- backward ----------------------------------------------------------------------------------------------
-// One row of a chunk: xhat and g = dy act'(pre)
-template <typename T>
-__device__ __forceinline__ void bwd_row(const Raw8<T>& xr, const Raw8<T>& dr, const Raw8<T>& rr, bool has_res, int act,
-                                        const float (&mean)[8], const float (&rstd)[8], const float (&ga)[8], const float (&be)[8],
-                                        float (&xh)[8], float (&g)[8]) {
-    constexpr bool EXACT = sizeof(T) == 4;
-    float q[8], u[8];
-    raw_f32(xr, xh);
+// One row of a chunk: x and g = dy act'(pre)
+template <typename T, int ACT, bool RES>
+__device__ __forceinline__ void bwd_row(const Raw8<T>& xr, const Raw8<T>& dr, const Raw8<T>& rr, const float (&sc)[8], const float (&sh)[8],
+                                        float (&x)[8], float (&g)[8]) {
+    float q[8];
+    raw_f32(xr, x);
     raw_f32(dr, g);
-    if (has_res) raw_f32(rr, q);
+    if (RES) raw_f32(rr, q);
+    if (ACT != CVG_ACT_NONE) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        // the same expression as the forward pass, so that the sign LeakyReLU takes is the same
-        const float d = xh[j] - mean[j];
-        u[j] = d * (ga[j] * rstd[j]) + be[j];
-        if (has_res) u[j] += q[j];
-        xh[j] = d * rstd[j];
-    }
-    if (act != CVG_ACT_NONE) {
-        act_slope8<EXACT>(u, act);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) g[j] *= u[j];
+        for (int j = 0; j < 8; ++j) {
+            float u = fmaf(x[j], sc[j], sh[j]);
+            if (RES) u += q[j];
+            g[j] *= act_slope<sizeof(T) == 4>(u, ACT);
+        }
     }
 }
 
-template <typename T, int R, bool RES>
-__global__ void __launch_bounds__(1024) gn_bwd_tile(const GnArgs a) {
+template <typename T, int ACT, int R, bool RES, int MAXT, int WAVES>
+__global__ void __launch_bounds__(MAXT, WAVES) gn_bwd_tile(const GnArgs a) {
     extern __shared__ float sm[];
     __shared__ float sums[2][GN_MAX_GROUPS];
     const Place p = gn_place(a);
     const size_t row0 = (size_t)p.b * a.HW + p.r0;
-    const int rows = p.r1 - p.r0, c = p.c0 + p.chunk * 8;
+    const int rows = p.r1 - p.r0, c = p.c0 + (p.live ? p.chunk * 8 : 0);
+    int gi[8];
+    chunk_groups(a, p, gi);
+    const float* gmean = a.stats + (size_t)p.b * a.G + p.g0;
+    const float* grstd = gmean + (size_t)a.B * a.G;
+    float mean[8], sc[8], sh[8], acc[2][8];
+    {
+        float ga[8], be[8];
+        load8<float>(a.gamma + c, ga);
+        load8<float>(a.beta + c, be);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) { mean[j] = gmean[gi[j]]; sc[j] = grstd[gi[j]]; }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            sc[j] *= ga[j];
+            sh[j] = fmaf(-mean[j], sc[j], be[j]);
+            acc[0][j] = acc[1][j] = 0.f;
+        }
+    }
     Raw8<T> xv[R], dv[R], qv[RES ? R : 1];
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-        const int r = p.ty + i * a.rpp;
-        raw_zero(xv[i]);
-        raw_zero(dv[i]);
-        if (RES) raw_zero(qv[RES ? i : 0]);
-        if (p.live && r < rows) {
-            raw_load(xv[i], (const T*)a.x + (row0 + r) * a.x_ld + c);
-            raw_load(dv[i], (const T*)a.dy + (row0 + r) * a.y_ld + c);
-            if (RES) raw_load(qv[RES ? i : 0], (const T*)a.res + (row0 + r) * a.res_ld + c);
-        }
+        const size_t r = row0 + min(p.ty + i * a.rpp, rows - 1);
+        raw_load(xv[i], (const T*)a.x + r * a.x_ld + c);
+        raw_load(dv[i], (const T*)a.dy + r * a.y_ld + c);
+        if (RES) raw_load(qv[RES ? i : 0], (const T*)a.res + r * a.res_ld + c);
     }
-    int gi[8];
-    chunk_groups(a, p, gi);
-    float mean[8], rstd[8], ga[8], be[8], acc[2][8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const size_t o = (size_t)p.b * a.G + p.g0 + gi[j];
-        mean[j] = a.stats[o];
-        rstd[j] = a.stats[(size_t)a.B * a.G + o];
-        ga[j] = p.live ? a.gamma[c + j] : 0.f;
-        be[j] = p.live ? a.beta[c + j] : 0.f;
-        acc[0][j] = acc[1][j] = 0.f;
-    }
+    const int mine = p.live ? rows : 0;
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-        if (p.live && p.ty + i * a.rpp < rows) {
-            float xh[8], g[8];
-            bwd_row<T>(xv[i], dv[i], qv[RES ? i : 0], RES, a.act, mean, rstd, ga, be, xh, g);
+        if (p.ty + i * a.rpp < mine) {
+            float x[8], g[8];
+            pin(xv[i]);
+            pin(dv[i]);
+            bwd_row<T, ACT, RES>(xv[i], dv[i], qv[RES ? i : 0], sc, sh, x, g);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) { acc[0][j] += g[j]; acc[1][j] += g[j] * xh[j]; }
+            for (int j = 0; j < 8; ++j) { acc[0][j] += g[j]; acc[1][j] += g[j] * (x[j] - mean[j]); }
         }
     }
-    column_sums<2>(a, p, acc, sm);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[1][j] *= grstd[gi[j]];         // sum of g xhat
+    column_parts<2>(a, p, acc, sm);
+    column_totals<2>(a, sm);
     const int width = a.nv * 8;
     float* o = a.part + ((size_t)p.b * a.tiles + p.tile) * 2 * a.C + p.c0;
     for (int t = threadIdx.x; t < p.nch; t += blockDim.x) {
@@ -329,28 +399,34 @@ __global__ void __launch_bounds__(1024) gn_bwd_tile(const GnArgs a) {
         o[a.C + t] = sm[(size_t)a.ent * width + t];
     }
     if (a.tiles > 1) return;
-    group_sums<2>(a, p, sm, a.gamma, sums);
-    if (!p.live) return;
+    group_sums<2>(a, p, sm, a.gamma, 1, sums);
     const float inv_n = 1.f / ((float)a.HW * (float)a.cg.d);
-    float A[8], Bq[8];
+    // dx = rstd (gamma g - mean(gamma g) - xhat mean(gamma g xhat)) = sc g + (x cd + c0)
+    float cd[8], c0[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) { A[j] = sums[0][gi[j]] * inv_n; Bq[j] = sums[1][gi[j]] * inv_n; }
+    for (int j = 0; j < 8; ++j) {
+        const float rstd = grstd[gi[j]];
+        cd[j] = -rstd * rstd * sums[1][gi[j]] * inv_n;
+        c0[j] = fmaf(-mean[j], cd[j], -rstd * sums[0][gi[j]] * inv_n);
+    }
 #pragma unroll
     for (int i = 0; i < R; ++i) {
         const int r = p.ty + i * a.rpp;
-        if (r < rows) {
-            float xh[8], g[8];
-            bwd_row<T>(xv[i], dv[i], qv[RES ? i : 0], RES, a.act, mean, rstd, ga, be, xh, g);
+        if (r < mine) {
+            float x[8], g[8];
+            pin(xv[i]);
+            pin(dv[i]);
+            bwd_row<T, ACT, RES>(xv[i], dv[i], qv[RES ? i : 0], sc, sh, x, g);
             if (a.dres) store8<T>((T*)a.dres + (row0 + r) * a.dres_ld + c, g);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) g[j] = rstd[j] * (ga[j] * g[j] - A[j] - xh[j] * Bq[j]);
+            for (int j = 0; j < 8; ++j) g[j] = fmaf(sc[j], g[j], fmaf(x[j], cd[j], c0[j]));
             store8<T>((T*)a.dx + (row0 + r) * a.dx_ld + c, g);
         }
     }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(512) gn_bwd_apply(const GnArgs a) {
+template <typename T, int ACT, bool RES>
+__global__ void __launch_bounds__(1024) gn_bwd_apply(const GnArgs a) {
     extern __shared__ float sm[];            // [2][slab channels]
     __shared__ float sums[2][GN_MAX_GROUPS];
     const Place p = gn_place(a);
@@ -360,62 +436,73 @@ __global__ void __launch_bounds__(512) gn_bwd_apply(const GnArgs a) {
         const int n = t >= width ? 1 : 0, ch = t - n * width;
         float s = 0.f;
         if (ch < p.nch)
+#pragma unroll 8
             for (int i = 0; i < a.tiles; ++i) s += q[((size_t)i * 2 + n) * a.C + ch];
         sm[t] = s;
     }
     __syncthreads();
-    group_sums<2>(a, p, sm, a.gamma, sums);  // (ent = 1 in this launch)
+    group_sums<2>(a, p, sm, a.gamma, 1, sums);   // (a.ent is 1 in this launch)
     if (!p.live) return;
     int gi[8];
     chunk_groups(a, p, gi);
     const int c = p.c0 + p.chunk * 8;
     const float inv_n = 1.f / ((float)a.HW * (float)a.cg.d);
-    float mean[8], rstd[8], ga[8], be[8], A[8], Bq[8];
+    float sc[8], sh[8], cd[8], c0[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         const size_t o = (size_t)p.b * a.G + p.g0 + gi[j];
-        mean[j] = a.stats[o];
-        rstd[j] = a.stats[(size_t)a.B * a.G + o];
-        ga[j] = a.gamma[c + j];
-        be[j] = a.beta[c + j];
-        A[j] = sums[0][gi[j]] * inv_n;
-        Bq[j] = sums[1][gi[j]] * inv_n;
+        const float rstd = a.stats[(size_t)a.B * a.G + o], mean = a.stats[o];
+        sc[j] = a.gamma[c + j] * rstd;
+        sh[j] = fmaf(-mean, sc[j], a.beta[c + j]);
+        cd[j] = -rstd * rstd * sums[1][gi[j]] * inv_n;
+        c0[j] = fmaf(-mean, cd[j], -rstd * sums[0][gi[j]] * inv_n);
     }
     const size_t row0 = (size_t)p.b * a.HW;
-    const bool has_res = a.res != nullptr;
-    for (int r = p.r0 + p.ty; r < p.r1; r += a.rpp) {
-        Raw8<T> xr, dr, rr;
-        raw_load(xr, (const T*)a.x + (row0 + r) * a.x_ld + c);
-        raw_load(dr, (const T*)a.dy + (row0 + r) * a.y_ld + c);
-        if (has_res) raw_load(rr, (const T*)a.res + (row0 + r) * a.res_ld + c); else raw_zero(rr);
-        float xh[8], g[8];
-        bwd_row<T>(xr, dr, rr, has_res, a.act, mean, rstd, ga, be, xh, g);
-        if (a.dres) store8<T>((T*)a.dres + (row0 + r) * a.dres_ld + c, g);
+    constexpr int U = sizeof(T) == 2 ? 4 : 2;
+    for (int r0 = p.r0 + p.ty; r0 < p.r1; r0 += U * a.rpp) {
+        Raw8<T> xr[U], dr[U], rr[U];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) g[j] = rstd[j] * (ga[j] * g[j] - A[j] - xh[j] * Bq[j]);
-        store8<T>((T*)a.dx + (row0 + r) * a.dx_ld + c, g);
+        for (int u = 0; u < U; ++u) {
+            const size_t r = row0 + min(r0 + u * a.rpp, p.r1 - 1);
+            raw_load(xr[u], (const T*)a.x + r * a.x_ld + c);
+            raw_load(dr[u], (const T*)a.dy + r * a.y_ld + c);
+            if (RES) raw_load(rr[u], (const T*)a.res + r * a.res_ld + c);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int r = r0 + u * a.rpp;
+            if (r < p.r1) {
+                float x[8], g[8];
+                bwd_row<T, ACT, RES>(xr[u], dr[u], rr[u], sc, sh, x, g);
+                if (a.dres) store8<T>((T*)a.dres + (row0 + r) * a.dres_ld + c, g);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) g[j] = fmaf(sc[j], g[j], fmaf(x[j], cd[j], c0[j]));
+                store8<T>((T*)a.dx + (row0 + r) * a.dx_ld + c, g);
+            }
+        }
     }
 }
 
-// dgamma / dbeta from the partial rows [P][2][C] (P = samples * tiles): 32 channels by 8 row lanes per workgroup
-__global__ void __launch_bounds__(256) gn_param_grad(const float* __restrict__ part, int P, int C, float* dgamma, float* dbeta) {
-    __shared__ float sm[2][8][32];
-    const int cl = threadIdx.x & 31, rl = threadIdx.x >> 5, c = blockIdx.x * 32 + cl;
-    float s0 = 0.f, s1 = 0.f;
-    if (c < C)
-        for (int i = rl; i < P; i += 8) {
-            s0 += part[(size_t)i * 2 * C + c];
-            s1 += part[((size_t)i * 2 + 1) * C + c];
-        }
-    sm[0][rl][cl] = s0;
-    sm[1][rl][cl] = s1;
-    __syncthreads();
-    if (rl < 2 && c < C) {
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) s += sm[rl][i][cl];
-        (rl ? dgamma : dbeta)[c] = s;
+// dgamma / dbeta from the partial rows [P][2][C] (P = samples * tiles): 16 columns by 64 row lanes per workgroup
+__global__ void __launch_bounds__(1024) gn_param_grad(const float* __restrict__ part, int P, int C, float* dgamma, float* dbeta) {
+    __shared__ float sm[64][17];
+    const int cl = threadIdx.x & 15, rl = threadIdx.x >> 4, col = blockIdx.x * 16 + cl;     // columns: dbeta, then dgamma
+    float s = 0.f;
+    if (col < 2 * C) {
+#pragma unroll 4
+        for (int i = rl; i < P; i += 64) s += part[(size_t)i * 2 * C + col];
     }
+    sm[rl][cl] = s;
+    __syncthreads();
+    if (threadIdx.x >= 64) return;
+    // one wave: 4 lanes per column, 16 rows each
+    const int c = threadIdx.x & 15, q = threadIdx.x >> 4, cc = blockIdx.x * 16 + c;
+    float t = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) t += sm[q * 16 + i][c];
+    t += __shfl_xor(t, 16, 64);
+    t += __shfl_xor(t, 32, 64);
+    if (q == 0 && cc < 2 * C) (cc < C ? dbeta : dgamma)[cc < C ? cc : cc - C] = t;
 }
 
 // ---- planning ----------------------------------------------------------------------------------------------
@@ -441,27 +528,41 @@ int check(const cvg_gn_desc* d, const char* who) {
     return 0;
 }
 
-Plan plan(const cvg_gn_desc* d, bool backward) {
+// Registers hold rmax chunks per thread and tensor: 1024 threads have 128 registers each, 512 have 256.
+Plan plan(const cvg_gn_desc* d, bool backward, bool res) {
     Plan p;
     const int cg = d->C / d->G, unit = cg / gcd(cg, 8);             // chunks of 8 channels that hold whole groups
     const int all = d->C / 8;
-    // slabs of 128 bytes per pixel row, or whatever one unit needs
-    const int want = d->dtype == CVG_BF16 ? 8 : 4;
-    p.nv = unit;
-    while (p.nv < want && p.nv + unit <= all) p.nv += unit;
-    p.nslab = ceil_div(all, p.nv);
-    const int rmax = (d->dtype == CVG_BF16 ? 8 : 4) / (backward ? 2 : 1);
+    const bool bf = d->dtype == CVG_BF16;
+    const int want = bf ? 8 : 4;                                    // 128 bytes of a pixel row
+    auto tmax = [](int nv) { return (nv & (nv - 1)) == 0 && nv <= 32 ? 1024 : 512; };   // (LDS rows where lanes do not fold)
+    auto rmax = [&](int threads) {
+        if (!backward) return (bf ? 8 : 4) * (threads <= 512 ? 2 : 1);
+        return (bf ? 16 : 8) / (res ? 2 : 1) / (threads <= 512 ? 1 : 4);
+    };
+    auto cap = [&](int nv) {                                        // rows one workgroup holds
+        int64_t best = 0;
+        for (int t = 512; t <= tmax(nv); t *= 2) { const int64_t c = (int64_t)(t / nv) * rmax(t); best = c > best ? c : best; }
+        return best;
+    };
+    int nv = unit;
+    while (nv < want && nv + unit <= all) nv += unit;
+    while (nv > unit && (d->HW > cap(nv) || (int64_t)d->B * ceil_div(all, nv) < 256)) nv -= unit;
+    const bool single = d->HW <= cap(nv);
+    if (!single) { nv = unit; while (nv < want && nv + unit <= all) nv += unit; }
+    p.nv = nv;
+    p.nslab = ceil_div(all, nv);
     p.threads = 256;
-    // (a chunk count that does not fold leaves one LDS row per row lane: 512 threads keep that within 32 KB)
-    const int tmax = (p.nv & (p.nv - 1)) == 0 && p.nv <= 32 ? 1024 : 512;
-    while (p.threads < tmax && (p.threads < p.nv || (int64_t)d->HW * p.nv > (int64_t)p.threads * rmax)) p.threads *= 2;
-    p.rpp = p.threads / p.nv;
-    int need = ceil_div(d->HW, p.rpp);
-    if (need > rmax) {
-        p.threads = p.nv <= 256 ? 256 : 512;
-        p.rpp = p.threads / p.nv;
-        need = rmax;
+    if (single) {
+        while (p.threads < tmax(nv) && (p.threads < nv || (int64_t)(p.threads / nv) * rmax(p.threads) < d->HW)) p.threads *= 2;
+    } else {
+        p.threads = nv <= 256 ? 256 : 512;
+        // enough tiles for every CU, otherwise as large as the registers allow
+        while (p.threads < tmax(nv) && (int64_t)d->B * p.nslab * ceil_div(d->HW, (p.threads / nv) * rmax(p.threads)) >= 1024) p.threads *= 2;
     }
+    p.rpp = p.threads / nv;
+    int need = ceil_div(d->HW, p.rpp);
+    if (need > rmax(p.threads)) need = rmax(p.threads);
     p.R = 1;
     while (p.R < need) p.R *= 2;
     p.rows_tile = min(d->HW, p.R * p.rpp);
@@ -479,6 +580,8 @@ void fill(GnArgs& a, const cvg_gn_desc* d, const Plan& p) {
     a.tiles = p.tiles; a.rows_tile = p.rows_tile; a.nslab = p.nslab; a.nv = p.nv; a.rpp = p.rpp; a.ent = entries(p);
     a.x_ld = d->x_ld ? d->x_ld : d->C; a.res_ld = d->res_ld ? d->res_ld : d->C; a.y_ld = d->y_ld ? d->y_ld : d->C;
     a.dx_ld = d->dx_ld ? d->dx_ld : d->C; a.dres_ld = d->dres_ld ? d->dres_ld : d->C;
+    a.seg = 1;
+    while (a.seg < 64 && a.seg < a.ent * (d->C / d->G)) a.seg *= 2;
     a.cg = make_fastdiv(d->C / d->G); a.nvd = make_fastdiv(p.nv); a.tiled = make_fastdiv(p.tiles); a.slabd = make_fastdiv(p.nslab);
 }
 
@@ -487,27 +590,44 @@ size_t ws_need(const cvg_gn_desc* d, const Plan& p, bool backward) {
     return p.tiles > 1 ? (size_t)d->B * d->G * p.tiles * 2 * 4 : 0;
 }
 
-template <typename T>
+// (the second number of a launch bound is waves per SIMD: 4 leave 128 registers)
+template <typename T, int ACT>
 void run_fwd(const GnArgs& a, const Plan& p, hipStream_t s) {
-    const int64_t blocks = (int64_t)a.B * p.nslab * p.tiles;
+    const int blocks = a.B * p.nslab * p.tiles;
     const size_t lds = (size_t)a.ent * p.nv * 8 * 4;
-    switch (p.R) {
-        case 1: gn_fwd_tile<T, 1><<<(int)blocks, p.threads, lds, s>>>(a); break;
-        case 2: gn_fwd_tile<T, 2><<<(int)blocks, p.threads, lds, s>>>(a); break;
-        case 4: gn_fwd_tile<T, 4><<<(int)blocks, p.threads, lds, s>>>(a); break;
-        default: gn_fwd_tile<T, 8><<<(int)blocks, p.threads, lds, s>>>(a); break;
-    }
+    constexpr bool B = sizeof(T) == 2;
+    if (p.R == 1) gn_fwd_tile<T, ACT, 1, 1024, 4><<<blocks, p.threads, lds, s>>>(a);
+    else if (p.R <= 4) gn_fwd_tile<T, ACT, 4, 1024, 4><<<blocks, p.threads, lds, s>>>(a);
+    else if (p.R == 8) gn_fwd_tile<T, ACT, 8, B ? 1024 : 512, 4><<<blocks, p.threads, lds, s>>>(a);
+    else if constexpr (B) gn_fwd_tile<T, ACT, 16, 512, 4><<<blocks, p.threads, lds, s>>>(a);
+    if (p.tiles > 1) gn_fwd_apply<T, ACT><<<blocks, p.threads, 0, s>>>(a);
 }
-template <typename T, bool RES>
-void run_bwd(const GnArgs& a, const Plan& p, hipStream_t s) {
-    const int64_t blocks = (int64_t)a.B * p.nslab * p.tiles;
+template <typename T, int ACT, bool RES>
+void run_bwd(GnArgs a, const Plan& p, hipStream_t s) {
+    const int blocks = a.B * p.nslab * p.tiles;
     const size_t lds = (size_t)a.ent * p.nv * 8 * 4 * 2;
-    switch (p.R) {
-        case 1: gn_bwd_tile<T, 1, RES><<<(int)blocks, p.threads, lds, s>>>(a); break;
-        case 2: gn_bwd_tile<T, 2, RES><<<(int)blocks, p.threads, lds, s>>>(a); break;
-        default: gn_bwd_tile<T, 4, RES><<<(int)blocks, p.threads, lds, s>>>(a); break;
+    constexpr bool B = sizeof(T) == 2;
+    constexpr int R1024 = (B ? 4 : 2) / (RES ? 2 : 1), R512 = 4 * R1024;
+    if (p.R == 1) gn_bwd_tile<T, ACT, 1, RES, 1024, 4><<<blocks, p.threads, lds, s>>>(a);
+    else if (p.R <= R1024) gn_bwd_tile<T, ACT, R1024, RES, 1024, 4><<<blocks, p.threads, lds, s>>>(a);
+    else if (p.R <= 2 * R1024) gn_bwd_tile<T, ACT, 2 * R1024, RES, 512, 2><<<blocks, p.threads, lds, s>>>(a);
+    else gn_bwd_tile<T, ACT, R512, RES, 512, 2><<<blocks, p.threads, lds, s>>>(a);
+    if (p.tiles > 1) {
+        a.ent = 1;
+        gn_bwd_apply<T, ACT, RES><<<blocks, p.threads, (size_t)2 * p.nv * 8 * 4, s>>>(a);
     }
 }
+template <typename T, int ACT>
+void run_bwd(const GnArgs& a, const Plan& p, hipStream_t s) {
+    if (a.res) run_bwd<T, ACT, true>(a, p, s); else run_bwd<T, ACT, false>(a, p, s);
+}
+#define GN_BY_ACT(run, T) \
+    switch (a.act) { \
+        case CVG_ACT_LRELU: run<T, CVG_ACT_LRELU>(a, p, st); break; \
+        case CVG_ACT_SILU: run<T, CVG_ACT_SILU>(a, p, st); break; \
+        case CVG_ACT_GELU: run<T, CVG_ACT_GELU>(a, p, st); break; \
+        default: run<T, CVG_ACT_NONE>(a, p, st); \
+    }
 
 }  // namespace
 
@@ -515,8 +635,11 @@ extern "C" {
 
 size_t cvg_gn_act_workspace(const cvg_gn_desc* d, int32_t backward) {
     if (check(d, "gn_act_workspace") != 0) return 0;
-    size_t n = ws_need(d, plan(d, false), false);
-    if (backward) n = n > ws_need(d, plan(d, true), true) ? n : ws_need(d, plan(d, true), true);
+    size_t n = ws_need(d, plan(d, false, false), false);
+    for (int res = 0; res < 2 && backward; ++res) {
+        const size_t b = ws_need(d, plan(d, true, res), true);
+        n = b > n ? b : n;
+    }
     return n;
 }
 
@@ -527,7 +650,7 @@ int cvg_gn_act_fwd(const cvg_gn_desc* d, const void* x, const void* res, void* y
     if (d->B == 0) return 0;
     CVG_CHECK(x && y, "gn_act_fwd: null tensor");
     CVG_CHECK(aligned16(x) && aligned16(res) && aligned16(y), "gn_act_fwd: tensors have to start at 16-byte borders");
-    const Plan p = plan(d, false);
+    const Plan p = plan(d, false, res != nullptr);
     CVG_CHECK((int64_t)d->B * p.nslab * p.tiles <= 0x7fffffff, "gn_act_fwd: too many tiles");
     const size_t need = ws_need(d, p, false);
     CVG_CHECK(need == 0 || (ws && ws_bytes >= need && ((uintptr_t)ws & 3) == 0), "gn_act_fwd: workspace of %zu bytes, need %zu", ws_bytes, need);
@@ -535,14 +658,8 @@ int cvg_gn_act_fwd(const cvg_gn_desc* d, const void* x, const void* res, void* y
     fill(a, d, p);
     a.x = x; a.res = res; a.y = y; a.stats = stats; a.gamma = gamma; a.beta = beta; a.part = (float*)ws;
     hipStream_t st = (hipStream_t)s;
-    if (d->dtype == CVG_BF16) run_fwd<bf16>(a, p, st); else run_fwd<float>(a, p, st);
+    if (d->dtype == CVG_BF16) { GN_BY_ACT(run_fwd, bf16) } else { GN_BY_ACT(run_fwd, float) }
     CVG_LAUNCH_CHECK();
-    if (p.tiles > 1) {
-        const int64_t blocks = (int64_t)d->B * p.nslab * p.tiles;
-        if (d->dtype == CVG_BF16) gn_fwd_apply<bf16><<<(int)blocks, p.threads, 0, st>>>(a);
-        else gn_fwd_apply<float><<<(int)blocks, p.threads, 0, st>>>(a);
-        CVG_LAUNCH_CHECK();
-    }
     return 0;
 }
 
@@ -554,7 +671,7 @@ int cvg_gn_act_bwd(const cvg_gn_desc* d, const void* dy, const void* x, const vo
     CVG_CHECK(d->B == 0 || (dy && x && dx && stats), "gn_act_bwd: null tensor");
     CVG_CHECK(aligned16(x) && aligned16(res) && aligned16(dy) && aligned16(dx) && aligned16(dres),
               "gn_act_bwd: tensors have to start at 16-byte borders");
-    const Plan p = plan(d, true);
+    const Plan p = plan(d, true, res != nullptr);
     CVG_CHECK((int64_t)d->B * p.nslab * p.tiles <= 0x7fffffff, "gn_act_bwd: too many tiles");
     const size_t need = ws_need(d, p, true);
     CVG_CHECK(need == 0 || (ws && ws_bytes >= need && ((uintptr_t)ws & 3) == 0), "gn_act_bwd: workspace of %zu bytes, need %zu", ws_bytes, need);
@@ -564,19 +681,10 @@ int cvg_gn_act_bwd(const cvg_gn_desc* d, const void* dy, const void* x, const vo
     a.part = (float*)ws;
     hipStream_t st = (hipStream_t)s;
     if (d->B > 0) {
-        if (d->dtype == CVG_BF16) { if (res) run_bwd<bf16, true>(a, p, st); else run_bwd<bf16, false>(a, p, st); }
-        else { if (res) run_bwd<float, true>(a, p, st); else run_bwd<float, false>(a, p, st); }
+        if (d->dtype == CVG_BF16) { GN_BY_ACT(run_bwd, bf16) } else { GN_BY_ACT(run_bwd, float) }
         CVG_LAUNCH_CHECK();
-        if (p.tiles > 1) {
-            const int64_t blocks = (int64_t)d->B * p.nslab * p.tiles;
-                a.ent = 1;
-            const size_t lds = (size_t)2 * p.nv * 8 * 4;
-            if (d->dtype == CVG_BF16) gn_bwd_apply<bf16><<<(int)blocks, p.threads, lds, st>>>(a);
-            else gn_bwd_apply<float><<<(int)blocks, p.threads, lds, st>>>(a);
-            CVG_LAUNCH_CHECK();
-        }
     }
-    gn_param_grad<<<ceil_div(d->C, 32), 256, 0, st>>>((const float*)ws, d->B * p.tiles, d->C, dgamma, dbeta);
+    gn_param_grad<<<ceil_div(2 * d->C, 16), 1024, 0, st>>>((const float*)ws, d->B * p.tiles, d->C, dgamma, dbeta);
     CVG_LAUNCH_CHECK();
     return 0;
 }

@@ -38,9 +38,29 @@ template <typename T>
 __device__ __forceinline__ void emit8(const Epi& e, int m, int n, int n_end, bool whole, float (&v)[8]) {
     constexpr bool EXACT = sizeof(T) == 4;
     if (!whole) {
+        float b[8], q[8];                // (all loads before the first use)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            b[j] = e.bias && n + j < n_end ? e.bias[n + j] : 0.f;
+            q[j] = e.res && n + j < n_end ? to_f32(((const T*)e.res)[(size_t)m * e.res_ld + n + j]) : 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] += b[j];
+        if (e.pre)
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (n + j < n_end) {
+                    if (e.pre_f32) ((float*)e.pre)[(size_t)m * e.pre_ld + n + j] = v[j];
+                    else ((T*)e.pre)[(size_t)m * e.pre_ld + n + j] = from_f32<T>(v[j]);
+                }
+        act_value8<EXACT>(v, e.act);
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-            if (n + j < n_end) emit<T>(e, m, n + j, v[j]);
+            if (n + j < n_end) {
+                const float o = v[j] + q[j];
+                if (e.out_f32) ((float*)e.out)[(size_t)m * e.out_ld + n + j] = o;
+                else ((T*)e.out)[(size_t)m * e.out_ld + n + j] = from_f32<T>(o);
+            }
         return;
     }
     if (e.bias) {
@@ -174,20 +194,22 @@ struct Operand {
 // Tile kernel: BM x BN per workgroup of WR x WC waves.  Two LDS stages of 128 bytes of k, filled by direct-to-LDS loads
 // two stages ahead; fragments are read one 16-k step ahead of the MFMAs that use them, across the stage border too, so
 // the one barrier of a stage sits between the last fragment reads of a stage and the MFMAs on them.
+template <typename T, int BM, int BN, int WR, int WC> struct TileLds {
+    static constexpr int STAGES = 2 * (BM + BN) * 128, EPI = WR * WC * 32 * (BN / WC * 4 + 16);
+    static constexpr int BYTES = STAGES > EPI ? STAGES : EPI;
+};
 template <typename T, int BM, int BN, int WR, int WC, bool ACOL, bool BCOL>
-__global__ void __launch_bounds__(WR * WC * 64) gemm_tile(GemmArgs a) {
+__device__ __forceinline__ void tile_body(const GemmArgs& a, int id, int slice, char* lds) {
     constexpr int NW = WR * WC, WM = BM / WR, WN = BN / WC, TI = WM / 32, TJ = WN / 32;
     typedef Operand<T, BM, NW, ACOL> OA;
     typedef Operand<T, BN, NW, BCOL> OB;
     typedef typename Elem<T>::frag frag;
     constexpr int BK = OA::BK, NS = BK / 16;
     constexpr int STAGE = OA::BYTES + OB::BYTES;
-    constexpr int EP = WN * 4 + 16, EPI = NW * 32 * EP;            // epilogue: 32 rows of the wave's columns, f32
-    __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE > EPI ? 2 * STAGE : EPI];
+    constexpr int EP = WN * 4 + 16;                                // epilogue: 32 rows of the wave's columns, f32
     // workgroups go round-robin over the 8 dies, each with its own L2: give every die a run of neighbouring tiles, walked
     // in strips of 4 tile rows
     const int nt = a.tiles_m * a.tiles_n;
-    int id = blockIdx.x;
     {
         const int per = nt >> 3, rest = nt & 7, x = id & 7, q = id >> 3;
         id = x * per + min(x, rest) + q;
@@ -195,7 +217,7 @@ __global__ void __launch_bounds__(WR * WC * 64) gemm_tile(GemmArgs a) {
     const int strip = id / (4 * a.tiles_n), in = id - strip * 4 * a.tiles_n;
     const int h_strip = min(4, a.tiles_m - strip * 4);
     const int m0 = (strip * 4 + in % h_strip) * BM, n0 = (in / h_strip) * BN;
-    const int k0 = blockIdx.y * a.k_split, k_len = min(a.K - k0, a.k_split);
+    const int k0 = slice * a.k_split, k_len = min(a.K - k0, a.k_split);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int wm = (wave / WC) * WM, wn = (wave % WC) * WN;
 
@@ -341,7 +363,7 @@ __global__ void __launch_bounds__(WR * WC * 64) gemm_tile(GemmArgs a) {
             load8<float>((const float*)(ep + (r + rl) * EP + cl * 4), v);
             if (m >= a.M || n >= a.N) continue;
             if (a.slab) {
-                float* o = a.slab + ((size_t)blockIdx.y * a.M + m) * a.N + n;
+                float* o = a.slab + ((size_t)slice * a.M + m) * a.N + n;
                 if (n + 8 <= a.N && (a.N & 3) == 0) store8<float>(o, v);
                 else
                     for (int j = 0; j < 8; ++j)
@@ -353,110 +375,190 @@ __global__ void __launch_bounds__(WR * WC * 64) gemm_tile(GemmArgs a) {
     }
 }
 
-// sums the slabs of a split contraction in order and applies the epilogue: 8 columns per thread
+template <typename T, int BM, int BN, int WR, int WC, bool ACOL, bool BCOL>
+__global__ void __launch_bounds__(WR * WC * 64) gemm_tile(const GemmArgs a) {
+    __shared__ __attribute__((aligned(1024))) char lds[TileLds<T, BM, BN, WR, WC>::BYTES];
+    tile_body<T, BM, BN, WR, WC, ACOL, BCOL>(a, blockIdx.x, blockIdx.y, lds);
+}
+
+// column sums of [P][N] partial rows: 32 columns by `blockDim / 32` row lanes
+__device__ __forceinline__ void sum_rows_body(const float* __restrict__ part, int P, int N, float* out, int blk, float (*sm)[32]) {
+    const int cl = threadIdx.x & 31, rl = threadIdx.x >> 5, lanes = blockDim.x >> 5, c = blk * 32 + cl;
+    float s = 0.f;
+    if (c < N) {
+#pragma unroll 8
+        for (int i = rl; i < P; i += lanes) s += part[(size_t)i * N + c];
+    }
+    sm[rl][cl] = s;
+    __syncthreads();
+    if (rl || c >= N) return;
+    s = 0.f;
+    for (int i = 0; i < lanes; ++i) s += sm[i][cl];
+    out[c] = s;
+}
+struct SumArgs { const float* part; float* out; int P, N; };
+
+// Both gradients of a layer in one launch: neither waits for the other, small ones do not fill the chip alone, and a
+// launch costs as much as they do.  The blocks behind the two products finish the bias gradient.
+template <typename T, int BM, int BN, int WR, int WC>
+__global__ void __launch_bounds__(WR * WC * 64) gemm_pair(const GemmArgs dx, const GemmArgs dw, int blocks_dx, int blocks_dw, const SumArgs db) {
+    __shared__ __attribute__((aligned(1024))) char lds[TileLds<T, BM, BN, WR, WC>::BYTES];
+    int blk = blockIdx.x;
+    if (blk < blocks_dx) {
+        const int nt = dx.tiles_m * dx.tiles_n, slice = blk / nt;
+        tile_body<T, BM, BN, WR, WC, false, true>(dx, blk - slice * nt, slice, lds);
+    } else if (blk < blocks_dx + blocks_dw) {
+        blk -= blocks_dx;
+        const int nt = dw.tiles_m * dw.tiles_n, slice = blk / nt;
+        tile_body<T, BM, BN, WR, WC, true, true>(dw, blk - slice * nt, slice, lds);
+    } else {
+        sum_rows_body(db.part, db.P, db.N, db.out, blk - blocks_dx - blocks_dw, (float (*)[32])lds);
+    }
+}
+__global__ void __launch_bounds__(256) sum_rows(const SumArgs a) {
+    __shared__ float sm[8][32];
+    sum_rows_body(a.part, a.P, a.N, a.out, blockIdx.x, sm);
+}
+
+// Sums the slabs of a split contraction and applies the epilogue.  A thread owns 8 columns of one row and one of zl runs
+// of consecutive slabs (few outputs would leave most of the chip idle otherwise); the runs are added in order.
 template <typename T>
-__global__ void __launch_bounds__(256) slab_sum(const GemmArgs a, int splits) {
-    const int n8 = (a.N + 7) / 8;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= (int64_t)a.M * n8) return;
-    const int m = (int)(i / n8), n = (int)(i % n8) * 8;
+__device__ __forceinline__ void slab_sum_body(const GemmArgs& a, int splits, int zl, int blk, float (*sm)[8]) {
+    const int n8 = (a.N + 7) / 8, per_blk = 256 / zl, lo = threadIdx.x % per_blk, zi = threadIdx.x / per_blk;
+    const int64_t i = (int64_t)blk * per_blk + lo;
+    const bool live = i < (int64_t)a.M * n8;
+    const int m = live ? (int)(i / n8) : 0, n = live ? (int)(i % n8) * 8 : 0;
     const float* p = a.slab + (size_t)m * a.N + n;
     const size_t stride = (size_t)a.M * a.N;
+    const int run = (splits + zl - 1) / zl, z1 = min(splits, (zi + 1) * run);
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (n + 8 <= a.N && (a.N & 3) == 0) {
-        for (int z = 0; z < splits; ++z) {
-            float q[8];
-            load8<float>(p + z * stride, q);
+    if (live) {
+        if (n + 8 <= a.N && (a.N & 3) == 0) {
+#pragma unroll 4
+            for (int z = zi * run; z < z1; ++z) {
+                float q[8];
+                load8<float>(p + z * stride, q);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] += q[j];
+                for (int j = 0; j < 8; ++j) v[j] += q[j];
+            }
+        } else {
+#pragma unroll 2
+            for (int z = zi * run; z < z1; ++z)
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (n + j < a.N) v[j] += p[z * stride + j];
         }
-    } else {
-        for (int z = 0; z < splits; ++z)
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (n + j < a.N) v[j] += p[z * stride + j];
     }
-    emit8<T>(a.e, m, n, a.N, a.vec && n + 8 <= a.N, v);
+    if (zl > 1) {
+        store8<float>(sm[threadIdx.x], v);
+        __syncthreads();
+        if (zi) return;
+        for (int q = 1; q < zl; ++q)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] += sm[q * per_blk + lo][j];
+    }
+    if (live) emit8<T>(a.e, m, n, a.N, a.vec && n + 8 <= a.N, v);
+}
+struct SlabJob { GemmArgs a; int splits, zl, blocks; };
+template <typename T>
+__global__ void __launch_bounds__(256) slab_sum(const SlabJob one, const SlabJob two) {
+    __shared__ __attribute__((aligned(16))) float sm[256][8];
+    if ((int)blockIdx.x < one.blocks) slab_sum_body<T>(one.a, one.splits, one.zl, blockIdx.x, sm);
+    else slab_sum_body<T>(two.a, two.splits, two.zl, blockIdx.x - one.blocks, sm);
 }
 
 // Rows that do not start on 16-byte borders (or are no whole number of 16 bytes long) are copied to padded rows first:
 // [rows][width] at pitch ld -> [rows][round_up(width, 8)], zeros behind.  One read and one write of an operand that the
 // product reads several times.
 template <typename T>
-__global__ void __launch_bounds__(256) pad_rows(const T* __restrict__ in, size_t ld, T* __restrict__ out, int rows, int width, int out_ld) {
+__device__ __forceinline__ void pad_body(const void* in, size_t ld, void* out, int rows, int width, int out_ld, int blk) {
     const int n8 = out_ld / 8;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t i = (int64_t)blk * 256 + threadIdx.x;
     if (i >= (int64_t)rows * n8) return;
     const int r = (int)(i / n8), c = (int)(i % n8) * 8;
+    const T* q = (const T*)in + (size_t)r * ld + c;
     float v[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = c + j < width ? to_f32(in[(size_t)r * ld + c + j]) : 0.f;
-    store8<T>(out + (size_t)r * out_ld + c, v);
+    for (int j = 0; j < 8; ++j) v[j] = c + j < width ? to_f32(q[j]) : 0.f;
+    store8<T>((T*)out + (size_t)r * out_ld + c, v);
 }
+struct PadJob { const void* in; void* out; size_t ld; int rows, width, out_ld, blocks; };
 
 // dz = dy act'(pre), rounded to T, into padded rows (zeros behind the N columns), and column sums of the unrounded values
 // over blocks of `rows_blk` rows.  A thread owns 8 columns; 32 column chunks by 8 row lanes per workgroup.
+struct DzJob {
+    const void *dy, *pre;
+    void* dz;                        // or null
+    float* part;                     // or null
+    size_t dy_ld, pre_ld;
+    int dz_ld, M, N, act, rows_blk, vec, col_blocks, blocks;
+};
 template <typename T, typename P>
-__global__ void __launch_bounds__(256) dz_colsum(const T* __restrict__ dy, size_t dy_ld, const P* __restrict__ pre, size_t pre_ld,
-                                                 T* dz, int dz_ld, float* part, int M, int N, int act, int rows_blk, int vec) {
+__device__ __forceinline__ void dz_body(const DzJob& a, int blk, float (*sm)[264]) {
     constexpr bool EXACT = sizeof(T) == 4;
-    __shared__ float sm[8][264];
-    const int cl = threadIdx.x & 31, rl = threadIdx.x >> 5, c = (blockIdx.x * 32 + cl) * 8;
+    constexpr int U = 4;             // rows in flight per thread
+    const int by = blk / a.col_blocks, bx = blk - by * a.col_blocks;
+    const int cl = threadIdx.x & 31, rl = threadIdx.x >> 5, c = (bx * 32 + cl) * 8;
     float s[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) s[j] = 0.f;
-    if (c < N) {
-        const bool whole = vec && c + 8 <= N;
-        const int64_t r1 = min((int64_t)M, ((int64_t)blockIdx.y + 1) * rows_blk);
-        for (int64_t r = (int64_t)blockIdx.y * rows_blk + rl; r < r1; r += 8) {
-            float g[8], q[8];
-            const T* gp = dy + (size_t)r * dy_ld + c;
-            const P* qp = pre + (size_t)r * pre_ld + c;
-            if (whole) {
-                load8<T>(gp, g);
-                if (act != CVG_ACT_NONE) load8<P>(qp, q);
-            } else {
+    if (c < a.N) {
+        const bool whole = a.vec && c + 8 <= a.N;
+        const int64_t r1 = min((int64_t)a.M, ((int64_t)by + 1) * a.rows_blk);
+        for (int64_t r0 = (int64_t)by * a.rows_blk + rl; r0 < r1; r0 += 8 * U) {
+            float g[U][8], q[U][8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    g[j] = c + j < N ? to_f32(gp[j]) : 0.f;
-                    q[j] = act != CVG_ACT_NONE && c + j < N ? to_f32(qp[j]) : 0.f;
+            for (int u = 0; u < U; ++u) {
+                const int64_t r = min(r0 + 8 * u, r1 - 1);
+                const T* gp = (const T*)a.dy + (size_t)r * a.dy_ld + c;
+                const P* qp = (const P*)a.pre + (size_t)r * a.pre_ld + c;
+                if (whole) {
+                    load8<T>(gp, g[u]);
+                    if (a.act != CVG_ACT_NONE) load8<P>(qp, q[u]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        g[u][j] = c + j < a.N ? to_f32(gp[j]) : 0.f;
+                        q[u][j] = a.act != CVG_ACT_NONE && c + j < a.N ? to_f32(qp[j]) : 0.f;
+                    }
                 }
             }
-            if (act != CVG_ACT_NONE) {
-                act_slope8<EXACT>(q, act);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) g[j] = c + j < N ? g[j] * q[j] : 0.f;
+            for (int u = 0; u < U; ++u) {
+                const int64_t r = r0 + 8 * u;
+                if (r >= r1) break;
+                if (a.act != CVG_ACT_NONE) {
+                    act_slope8<EXACT>(q[u], a.act);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) g[u][j] = c + j < a.N ? g[u][j] * q[u][j] : 0.f;
+                }
+                if (a.dz) store8<T>((T*)a.dz + (size_t)r * a.dz_ld + c, g[u]);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) s[j] += g[u][j];
             }
-            if (dz) store8<T>(dz + (size_t)r * dz_ld + c, g);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) s[j] += g[j];
         }
     }
-    if (!part) return;
+    if (!a.part) return;
 #pragma unroll
     for (int j = 0; j < 8; ++j) sm[rl][cl * 8 + j] = s[j];
     __syncthreads();
-    const int col = blockIdx.x * 256 + threadIdx.x;
-    if (col >= N) return;
+    const int col = bx * 256 + threadIdx.x;
+    if (col >= a.N) return;
     float t = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) t += sm[i][threadIdx.x];
-    part[(size_t)blockIdx.y * N + col] = t;
+    a.part[(size_t)by * a.N + col] = t;
 }
-// [P][N] -> column sums: 32 columns by 8 row lanes
-__global__ void __launch_bounds__(256) sum_rows(const float* __restrict__ part, int P, int N, float* out) {
-    __shared__ float sm[8][32];
-    const int cl = threadIdx.x & 31, rl = threadIdx.x >> 5, c = blockIdx.x * 32 + cl;
-    float s = 0.f;
-    if (c < N)
-        for (int i = rl; i < P; i += 8) s += part[(size_t)i * N + c];
-    sm[rl][cl] = s;
-    __syncthreads();
-    if (rl || c >= N) return;
-    s = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) s += sm[i][cl];
-    out[c] = s;
+
+// What has to happen before the products, in one launch: dz and the bias gradient's partial sums, padded copies
+template <typename T, typename P>
+__global__ void __launch_bounds__(256) prepare(const DzJob dz, const PadJob p0, const PadJob p1) {
+    __shared__ float sm[8][264];
+    int blk = blockIdx.x;
+    if (blk < dz.blocks) { dz_body<T, P>(dz, blk, sm); return; }
+    blk -= dz.blocks;
+    if (blk < p0.blocks) pad_body<T>(p0.in, p0.ld, p0.out, p0.rows, p0.width, p0.out_ld, blk);
+    else pad_body<T>(p1.in, p1.ld, p1.out, p1.rows, p1.width, p1.out_ld, blk - p0.blocks);
 }
 
 __global__ void __launch_bounds__(256) zero_rows(char* out, size_t pitch, int rows, int width, int es) {
@@ -496,45 +598,55 @@ int check(const cvg_linear_desc* d, const char* who) {
 // BM x BN tile takes `mfma` cycles of its matrix units, never less than the load latency a two-stage pipeline leaves
 // exposed; workgroups beyond one round queue up; K ranges add their f32 slabs (written and read once at ~2000 bytes per
 // cycle chip-wide) and a launch.
-struct Tile { int cfg, splits, k_split; };
+struct Tile { int cfg, splits, k_split; double t; };
 struct TileShape { int bm, bn, occ; double mfma; };
-Tile choose(int dtype, int64_t M, int64_t N, int64_t K) {
-    static const TileShape bf[3] = {{256, 256, 1, 2048 / .8}, {128, 128, 2, 512 / .6}, {64, 64, 4, 128 / .4}};
-    static const TileShape f3[3] = {{0, 0, 0, 0}, {128, 128, 2, 4096 / .85}, {64, 64, 3, 1024 / .7}};
-    const TileShape* sh = dtype == CVG_BF16 ? bf : f3;
+const TileShape TILES[2][3] = {{{0, 0, 0, 0}, {128, 128, 2, 4096 / .85}, {64, 64, 3, 1024 / .7}},
+                               {{256, 256, 1, 2048 / .8}, {128, 128, 2, 512 / .6}, {64, 64, 4, 128 / .4}}};
+Tile choose_split(int dtype, int c, int64_t M, int64_t N, int64_t K) {
+    const TileShape& sh = TILES[dtype == CVG_BF16][c];
     const int bk = dtype == CVG_BF16 ? 64 : 32;
     const int64_t stages = (K + bk - 1) / bk;
-    Tile best{2, 1, (int)round_up(K, bk)};
-    double best_t = 1e300;
-    for (int c = 0; c < 3; ++c) {
-        if (!sh[c].bm) continue;
-        const int64_t tiles = ((M + sh[c].bm - 1) / sh[c].bm) * ((N + sh[c].bn - 1) / sh[c].bn);
-        for (int64_t sp = 1; sp <= 64; sp *= 2) {
-            const int64_t per = (stages + sp - 1) / sp;
-            if (sp > 1 && (per < 2 || tiles * sp > 2048)) break;
-            const int64_t real = (stages + per - 1) / per;             // ranges that hold any k
-            const int64_t wgs = tiles * real, per_cu = (wgs + 255) / 256;
-            const int64_t rounds = (per_cu + sh[c].occ - 1) / sh[c].occ;
-            const int64_t together = per_cu < sh[c].occ ? per_cu : sh[c].occ;
-            double stage = sh[c].mfma * together;
-            if (stage < 700) stage = 700;
-            double t = rounds * (per * stage + 4000);
-            if (real > 1) t += 6000 + (double)real * M * N * 8 / 2000;
-            if (t < best_t) { best_t = t; best = Tile{c, (int)real, (int)(per * bk)}; }
-        }
+    Tile best{c, 1, (int)round_up(K, bk), 1e300};
+    const int64_t tiles = ((M + sh.bm - 1) / sh.bm) * ((N + sh.bn - 1) / sh.bn);
+    for (int64_t sp = 1; sp <= 64; sp *= 2) {
+        const int64_t per = (stages + sp - 1) / sp;
+        if (sp > 1 && (per < 2 || tiles * sp > 2048)) break;
+        const int64_t real = (stages + per - 1) / per;                 // ranges that hold any k
+        const int64_t wgs = tiles * real, per_cu = (wgs + 255) / 256;
+        const int64_t rounds = (per_cu + sh.occ - 1) / sh.occ;
+        const int64_t together = per_cu < sh.occ ? per_cu : sh.occ;
+        double stage = sh.mfma * together;
+        if (stage < 700) stage = 700;
+        double t = rounds * (per * stage + 4000);
+        if (real > 1) t += 6000 + (double)real * M * N * 8 / 2000;
+        if (t < best.t) best = Tile{c, (int)real, (int)(per * bk), t};
     }
     return best;
 }
-size_t slab_bytes(int dtype, int64_t M, int64_t N, int64_t K) {
-    if (M == 0 || N == 0 || K == 0) return 0;                    // (no rows: nothing is multiplied)
-    const Tile t = choose(dtype, M, N, K);
-    return t.splits > 1 ? (size_t)t.splits * M * N * 4 : 0;
+Tile choose(int dtype, int64_t M, int64_t N, int64_t K) {
+    Tile best{2, 1, 0, 1e301};
+    for (int c = dtype == CVG_BF16 ? 0 : 1; c < 3; ++c) {
+        const Tile t = choose_split(dtype, c, M, N, K);
+        if (t.t < best.t) best = t;
+    }
+    return best;
 }
+// Both gradients with one tile shape in one launch, or (cfg 0) apart
+struct PairPlan { bool together; Tile dx, dw; };
+PairPlan choose_pair(const cvg_linear_desc* d) {
+    PairPlan p{false, choose(d->dtype, d->M, d->K, d->N), choose(d->dtype, d->N, d->K, d->M)};
+    if (p.dx.cfg == 0 || p.dw.cfg == 0) return p;
+    p.together = true;
+    if (p.dx.cfg != p.dw.cfg) {
+        const Tile a = choose_split(d->dtype, p.dw.cfg, d->M, d->K, d->N), b = choose_split(d->dtype, p.dx.cfg, d->N, d->K, d->M);
+        if (a.t + p.dw.t < b.t + p.dx.t) p.dx = a; else p.dw = b;
+    }
+    return p;
+}
+size_t slab_of(const Tile& t, int64_t M, int64_t N) { return t.splits > 1 ? round_up((size_t)t.splits * M * N * 4, 256) : 0; }
 
 template <typename T, int BM, int BN, int WR, int WC>
 void launch_tile(GemmArgs& a, bool acol, bool bcol, int splits, hipStream_t s) {
-    a.tiles_m = ceil_div(a.M, BM);
-    a.tiles_n = ceil_div(a.N, BN);
     const dim3 grid(a.tiles_m * a.tiles_n, splits);
     if (!acol && !bcol) gemm_tile<T, BM, BN, WR, WC, false, false><<<grid, WR * WC * 64, 0, s>>>(a);
     else if (!acol) gemm_tile<T, BM, BN, WR, WC, false, true><<<grid, WR * WC * 64, 0, s>>>(a);
@@ -547,22 +659,19 @@ bool fits(const Rows& r, size_t es) { return aligned16(r.p) && r.ld * es % 16 ==
 size_t padded_bytes(int64_t rows, int64_t width, size_t es) { return round_up((size_t)rows * round_up(width, 8) * es, 256); }
 
 template <typename T>
-int pad(Rows& r, char*& ws, hipStream_t s) {
-    if (fits(r, sizeof(T))) return 0;
-    T* out = (T*)ws;
+PadJob pad_job(Rows& r, char*& ws) {
+    PadJob j{};
+    if (fits(r, sizeof(T))) return j;
+    j.in = r.p; j.ld = r.ld; j.out = ws; j.rows = (int)r.rows; j.width = (int)r.width; j.out_ld = (int)round_up(r.width, 8);
+    j.blocks = ceil_div(r.rows * (j.out_ld / 8), 256);
     ws += padded_bytes(r.rows, r.width, sizeof(T));
-    const int ld = (int)round_up(r.width, 8);
-    pad_rows<T><<<ceil_div(r.rows * (ld / 8), 256), 256, 0, s>>>((const T*)r.p, r.ld, out, (int)r.rows, (int)r.width, ld);
-    CVG_LAUNCH_CHECK();
-    r.p = out;
-    r.ld = ld;
-    r.width = ld;
-    return 0;
+    r.p = j.out; r.ld = j.out_ld; r.width = j.out_ld;
+    return j;
 }
 
 // D = A B^T with A, B fit for the tile kernel; acol / bcol: the operand's rows run along k
 template <typename T>
-int gemm(const Rows& A, bool acol, const Rows& B, bool bcol, int64_t M, int64_t N, int64_t K, const Epi& e, char* slab, hipStream_t s) {
+GemmArgs gemm_args(const Rows& A, bool acol, const Rows& B, bool bcol, int64_t M, int64_t N, int64_t K, const Epi& e, const Tile& t, char*& ws) {
     GemmArgs a{};
     a.A = A.p; a.B = B.p; a.lda = A.ld; a.ldb = B.ld;
     a.M = (int)M; a.N = (int)N; a.K = (int)K; a.e = e;
@@ -571,9 +680,35 @@ int gemm(const Rows& A, bool acol, const Rows& B, bool bcol, int64_t M, int64_t 
     const size_t oes = e.out_f32 ? 4 : sizeof(T), pes = e.pre_f32 ? 4 : sizeof(T);
     a.vec = aligned16(e.out) && e.out_ld * oes % 16 == 0 && (!e.pre || (aligned16(e.pre) && e.pre_ld * pes % 16 == 0)) &&
             (!e.res || (aligned16(e.res) && e.res_ld * sizeof(T) % 16 == 0)) && aligned16(e.bias);
-    const Tile t = choose(Elem<T>::DT, M, N, K);
+    const TileShape& sh = TILES[sizeof(T) == 2][t.cfg];
+    a.tiles_m = ceil_div(M, sh.bm);
+    a.tiles_n = ceil_div(N, sh.bn);
     a.k_split = t.k_split;
-    a.slab = t.splits > 1 ? (float*)slab : nullptr;
+    a.slab = t.splits > 1 ? (float*)ws : nullptr;
+    ws += slab_of(t, M, N);
+    return a;
+}
+template <typename T>
+SlabJob slab_job(const GemmArgs& a, const Tile& t) {
+    SlabJob j{};
+    if (t.splits <= 1) return j;
+    j.a = a;
+    j.splits = t.splits;
+    const int64_t outs = (int64_t)a.M * ((a.N + 7) / 8);
+    j.zl = 1;
+    while (j.zl < 16 && outs * j.zl < 131072 && t.splits >= 4 * j.zl) j.zl *= 2;
+    j.blocks = ceil_div(outs, 256 / j.zl);
+    return j;
+}
+template <typename T>
+int sum_slabs(const SlabJob& one, const SlabJob& two, hipStream_t s) {
+    if (one.blocks + two.blocks == 0) return 0;
+    slab_sum<T><<<one.blocks + two.blocks, 256, 0, s>>>(one, two);
+    CVG_LAUNCH_CHECK();
+    return 0;
+}
+template <typename T>
+int multiply(GemmArgs& a, bool acol, bool bcol, const Tile& t, hipStream_t s) {
     if (t.cfg == 0) {
         if constexpr (sizeof(T) == 2) launch_tile<T, 256, 256, 2, 4>(a, acol, bcol, t.splits, s);
     } else if (t.cfg == 1) {
@@ -582,96 +717,113 @@ int gemm(const Rows& A, bool acol, const Rows& B, bool bcol, int64_t M, int64_t 
         launch_tile<T, 64, 64, 2, 2>(a, acol, bcol, t.splits, s);
     }
     CVG_LAUNCH_CHECK();
-    if (t.splits > 1) {
-        slab_sum<T><<<ceil_div(M * ((N + 7) / 8), 256), 256, 0, s>>>(a, t.splits);
-        CVG_LAUNCH_CHECK();
-    }
-    return 0;
+    return sum_slabs<T>(slab_job<T>(a, t), SlabJob{}, s);
 }
 
-// Workspaces: padded copies first, then slabs.  The sizes do not depend on pitches or alignment, so one workspace serves
-// every call of the same shape.
+// Workspaces: dz, partial column sums, padded copies, slabs.  The sizes do not depend on pitches or alignment, so one
+// workspace serves every call of the same shape.
 size_t fwd_ws(const cvg_linear_desc* d) {
+    if (d->M == 0) return 0;
     const size_t es = es_of(d->dtype);
-    return padded_bytes(d->M, d->K, es) + padded_bytes(d->N, d->K, es) + slab_bytes(d->dtype, d->M, d->N, d->K);
+    return padded_bytes(d->M, d->K, es) + padded_bytes(d->N, d->K, es) + slab_of(choose(d->dtype, d->M, d->N, d->K), d->M, d->N);
 }
 int dz_rows_blk(const cvg_linear_desc* d) {
-    // about 2048 workgroups where there are rows enough, at least 8 rows each
+    // about 2048 workgroups where there are rows enough, at least 32 rows each
     const int64_t cols = ceil_div(d->N, 256);
     int64_t blks = 2048 / cols > 0 ? 2048 / cols : 1;
-    if (blks > 256) blks = 256;
+    if (blks > 128) blks = 128;
     const int64_t rb = ceil_div(d->M, blks);
-    return (int)(rb < 8 ? 8 : round_up(rb, 8));
+    return (int)(rb < 32 ? 32 : round_up(rb, 32));
 }
 size_t part_bytes(const cvg_linear_desc* d) { return round_up((size_t)ceil_div(d->M, dz_rows_blk(d)) * d->N * 4, 256); }
 size_t bwd_ws(const cvg_linear_desc* d) {
+    if (d->M == 0) return 0;
     const size_t es = es_of(d->dtype);
+    const PairPlan p = choose_pair(d);
     return padded_bytes(d->M, d->N, es) + part_bytes(d) + padded_bytes(d->N, d->K, es) + padded_bytes(d->M, d->K, es) +
-           max_sz(slab_bytes(d->dtype, d->M, d->K, d->N), slab_bytes(d->dtype, d->N, d->K, d->M));
+           slab_of(p.dx, d->M, d->K) + slab_of(p.dw, d->N, d->K);
 }
 
 template <typename T>
 int forward(const cvg_linear_desc* d, const void* x, const void* w, const float* bias, const void* res, void* y, void* pre, char* ws,
             hipStream_t s) {
     Rows X{x, ld_of(d->x_ld, d->K), d->M, d->K}, W{w, ld_of(d->w_ld, d->K), d->N, d->K};
-    if (pad<T>(X, ws, s) != 0 || pad<T>(W, ws, s) != 0) return -1;
+    const PadJob p0 = pad_job<T>(X, ws), p1 = pad_job<T>(W, ws);
+    if (p0.blocks + p1.blocks) {
+        prepare<T, T><<<p0.blocks + p1.blocks, 256, 0, s>>>(DzJob{}, p0, p1);
+        CVG_LAUNCH_CHECK();
+    }
     Epi e{};
     e.bias = bias; e.res = res; e.pre = pre; e.out = y; e.act = d->act;
     e.out_f32 = 0; e.pre_f32 = sizeof(T) == 2 && d->pre_dtype == CVG_F32;
     e.res_ld = ld_of(d->res_ld, d->N); e.pre_ld = ld_of(d->pre_ld, d->N); e.out_ld = ld_of(d->y_ld, d->N);
-    return gemm<T>(X, false, W, false, d->M, d->N, d->K, e, ws, s);
+    const Tile t = choose(Elem<T>::DT, d->M, d->N, d->K);
+    GemmArgs a = gemm_args<T>(X, false, W, false, d->M, d->N, d->K, e, t, ws);
+    return multiply<T>(a, false, false, t, s);
 }
 
+// M > 0
 template <typename T, typename P>
 int backward(const cvg_linear_desc* d, const void* dy, const void* x, const void* w, const void* pre, void* dx, void* dw,
              float* dbias, char* ws, hipStream_t s) {
     Rows G{dy, ld_of(d->dy_ld, d->N), d->M, d->N};
-    const bool act = d->act != CVG_ACT_NONE, products = (dx || dw) && d->M > 0;
+    const bool act = d->act != CVG_ACT_NONE, products = dx || dw;
     const bool copy = products && (act || !fits(G, sizeof(T)));
-    if (d->M > 0 && (dbias || copy)) {
-        const int rb = dz_rows_blk(d), blks = ceil_div(d->M, rb);
-        const size_t pld = ld_of(d->pre_ld, d->N);
-        T* dz = copy ? (T*)ws : nullptr;
-        ws += copy ? padded_bytes(d->M, d->N, sizeof(T)) : 0;
-        float* part = dbias ? (float*)ws : nullptr;
-        ws += dbias ? part_bytes(d) : 0;
-        const int vec = aligned16(dy) && G.ld * sizeof(T) % 16 == 0 && (!act || (aligned16(pre) && pld * sizeof(P) % 16 == 0));
-        const int dz_ld = (int)round_up(d->N, 8);
-        dz_colsum<T, P><<<dim3(ceil_div(d->N, 256), blks), 256, 0, s>>>((const T*)dy, G.ld, (const P*)pre, pld, dz, dz_ld, part, d->M,
-                                                                      d->N, d->act, rb, vec);
-        CVG_LAUNCH_CHECK();
+    DzJob z{};
+    SumArgs sum{};
+    if (dbias || copy) {
+        z.dy = dy; z.dy_ld = G.ld; z.pre = pre; z.pre_ld = ld_of(d->pre_ld, d->N);
+        z.M = d->M; z.N = d->N; z.act = d->act; z.dz_ld = (int)round_up(d->N, 8);
+        z.rows_blk = dz_rows_blk(d);
+        z.col_blocks = ceil_div(d->N, 256);
+        z.blocks = z.col_blocks * ceil_div(d->M, z.rows_blk);
+        z.vec = aligned16(dy) && G.ld * sizeof(T) % 16 == 0 && (!act || (aligned16(pre) && z.pre_ld * sizeof(P) % 16 == 0));
+        if (copy) {
+            z.dz = ws;
+            ws += padded_bytes(d->M, d->N, sizeof(T));
+            G.p = z.dz; G.ld = z.dz_ld; G.width = z.dz_ld;
+        }
         if (dbias) {
-            sum_rows<<<ceil_div(d->N, 32), 256, 0, s>>>(part, blks, d->N, dbias);
-            CVG_LAUNCH_CHECK();
+            z.part = (float*)ws;
+            ws += part_bytes(d);
+            sum.part = z.part; sum.out = dbias; sum.N = d->N; sum.P = ceil_div(d->M, z.rows_blk);
         }
-        if (copy) { G.p = dz; G.ld = dz_ld; G.width = dz_ld; }
-    } else if (dbias) {
-        sum_rows<<<ceil_div(d->N, 32), 256, 0, s>>>(nullptr, 0, d->N, dbias);
+    }
+    Rows W{w, ld_of(d->w_ld, d->K), d->N, d->K}, X{x, ld_of(d->x_ld, d->K), d->M, d->K};
+    const PadJob p0 = dx ? pad_job<T>(W, ws) : PadJob{}, p1 = dw ? pad_job<T>(X, ws) : PadJob{};
+    if (z.blocks + p0.blocks + p1.blocks) {
+        prepare<T, P><<<z.blocks + p0.blocks + p1.blocks, 256, 0, s>>>(z, p0, p1);
         CVG_LAUNCH_CHECK();
     }
-    if (dx && d->M > 0) {
-        Rows W{w, ld_of(d->w_ld, d->K), d->N, d->K};
-        char* at = ws;
-        if (pad<T>(W, at, s) != 0) return -1;
-        Epi e{};
-        e.out = dx; e.out_ld = ld_of(d->dx_ld, d->K);
-        if (gemm<T>(G, false, W, true, d->M, d->K, d->N, e, at, s) != 0) return -1;
+    const PairPlan plan = choose_pair(d);
+    Epi ex{}, ew{};
+    ex.out = dx; ex.out_ld = ld_of(d->dx_ld, d->K);
+    ew.out = dw; ew.out_ld = ld_of(d->dw_ld, d->K); ew.out_f32 = sizeof(T) == 2 && d->dw_dtype == CVG_F32;
+    GemmArgs ax = gemm_args<T>(G, false, W, true, d->M, d->K, d->N, ex, plan.dx, ws);
+    GemmArgs aw = gemm_args<T>(G, true, X, true, d->N, d->K, d->M, ew, plan.dw, ws);
+    const int sum_blocks = dbias ? ceil_div(d->N, 32) : 0;
+    if (plan.together && products) {
+        const int bx = dx ? ax.tiles_m * ax.tiles_n * plan.dx.splits : 0, bw = dw ? aw.tiles_m * aw.tiles_n * plan.dw.splits : 0;
+        if (plan.dx.cfg == 1) gemm_pair<T, 128, 128, 2, 2><<<bx + bw + sum_blocks, 256, 0, s>>>(ax, aw, bx, bw, sum);
+        else gemm_pair<T, 64, 64, 2, 2><<<bx + bw + sum_blocks, 256, 0, s>>>(ax, aw, bx, bw, sum);
+        CVG_LAUNCH_CHECK();
+        return sum_slabs<T>(dx ? slab_job<T>(ax, plan.dx) : SlabJob{}, dw ? slab_job<T>(aw, plan.dw) : SlabJob{}, s);
     }
-    if (dw) {
-        Epi e{};
-        e.out = dw; e.out_ld = ld_of(d->dw_ld, d->K); e.out_f32 = sizeof(T) == 2 && d->dw_dtype == CVG_F32;
-        if (d->M == 0) {
-            // no rows: the sum is zero
-            zero_rows<<<ceil_div((int64_t)d->N * d->K, 256), 256, 0, s>>>((char*)dw, e.out_ld * (d->dw_dtype == CVG_F32 ? 4 : 2), d->N, d->K,
-                                                                          d->dw_dtype == CVG_F32 ? 4 : 2);
-            CVG_LAUNCH_CHECK();
-            return 0;
-        }
-        Rows X{x, ld_of(d->x_ld, d->K), d->M, d->K};
-        char* at = ws;
-        if (pad<T>(X, at, s) != 0) return -1;
-        if (gemm<T>(G, true, X, true, d->N, d->K, d->M, e, at, s) != 0) return -1;
+    if (sum_blocks) {
+        sum_rows<<<sum_blocks, 256, 0, s>>>(sum);
+        CVG_LAUNCH_CHECK();
     }
+    if (dx && multiply<T>(ax, false, true, plan.dx, s) != 0) return -1;
+    if (dw && multiply<T>(aw, true, true, plan.dw, s) != 0) return -1;
+    return 0;
+}
+
+// no rows: the sums are zero
+int backward_empty(const cvg_linear_desc* d, void* dw, float* dbias, hipStream_t s) {
+    const int es = d->dw_dtype == CVG_F32 ? 4 : 2;
+    if (dw) zero_rows<<<ceil_div((int64_t)d->N * d->K, 256), 256, 0, s>>>((char*)dw, ld_of(d->dw_ld, d->K) * es, d->N, d->K, es);
+    if (dbias) zero_rows<<<ceil_div(d->N, 256), 256, 0, s>>>((char*)dbias, 0, 1, d->N, 4);
+    CVG_LAUNCH_CHECK();
     return 0;
 }
 
@@ -713,8 +865,9 @@ int cvg_linear_act_bwd(const cvg_linear_desc* d, const void* dy, const void* x, 
     CVG_CHECK((uintptr_t)pre % es_of(d->pre_dtype) == 0 && (uintptr_t)dbias % 4 == 0, "linear_act_bwd: misaligned tensor");
     CVG_CHECK((uintptr_t)dw % es_of(d->dw_dtype) == 0, "linear_act_bwd: misaligned dw");
     const size_t need = bwd_ws(d);
-    CVG_CHECK(ws && ws_bytes >= need && aligned16(ws), "linear_act_bwd: workspace of %zu bytes, need %zu", ws_bytes, need);
+    CVG_CHECK(need == 0 || (ws && ws_bytes >= need && aligned16(ws)), "linear_act_bwd: workspace of %zu bytes, need %zu", ws_bytes, need);
     hipStream_t st = (hipStream_t)s;
+    if (d->M == 0) return backward_empty(d, dw, dbias, st);
     char* w0 = (char*)ws;
     if (d->dtype == CVG_F32) return backward<float, float>(d, dy, x, w, pre, dx, dw, dbias, w0, st);
     if (d->pre_dtype == CVG_F32) return backward<bf16, float>(d, dy, x, w, pre, dx, dw, dbias, w0, st);

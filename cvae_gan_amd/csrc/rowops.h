@@ -85,3 +85,12 @@ __device__ __forceinline__ void raw_f32(const Raw8<float>& r, float (&v)[8]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) { v[i] = __uint_as_float(r.a[i]); v[4 + i] = __uint_as_float(r.b[i]); }
 }
+// (exact for values that came from such elements)
+__device__ __forceinline__ void raw_pack(Raw8<bf16>& r, const float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.a[i] = (__float_as_uint(v[2 * i]) >> 16) | (__float_as_uint(v[2 * i + 1]) & 0xffff0000u);
+}
+__device__ __forceinline__ void raw_pack(Raw8<float>& r, const float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { r.a[i] = __float_as_uint(v[i]); r.b[i] = __float_as_uint(v[4 + i]); }
+}

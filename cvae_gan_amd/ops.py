@@ -336,19 +336,20 @@ def _need(ok, fmt, *args):
         raise CvgError(fmt % args)
 
 
-def _like(name, t, ref_name, ref, shape=None, dtype=None):
-    """t (when given) has ref's device, and the given shape / dtype (default: ref's)."""
-    if t is None:
+def _is(name, t, shape, dtype, device):
+    """t (when given) has this shape, type and device."""
+    if t is None or (t.shape == shape and t.dtype == dtype and t.device == device):
         return
-    shape = ref.shape if shape is None else shape
-    dtype = ref.dtype if dtype is None else dtype
     _need(tuple(t.shape) == tuple(shape), "%s has shape %s, expected %s", name, tuple(t.shape), tuple(shape))
     _need(t.dtype == dtype, "%s is %s, expected %s", name, t.dtype, dtype)
-    _need(t.device == ref.device, "%s is on %s, %s on %s", name, t.device, ref_name, ref.device)
+    _need(False, "%s is on %s, the other operands on %s", name, t.device, device)
 
 
-def _dense(name, t):
-    _need(t is None or t.is_contiguous(), "%s has to be contiguous", name)
+def _vec(name, t, shape, device):
+    """A dense f32 tensor."""
+    _is(name, t, shape, torch.float32, device)
+    if t is not None and not t.is_contiguous():
+        raise CvgError("%s has to be contiguous" % name)
 
 
 def _pitch(name, t):
@@ -376,12 +377,15 @@ def _pitch(name, t):
 
 
 def _launch(fn, dev, *args):
-    _need(dev.type == "cuda", "cvae_gan_amd ops need device tensors")
-    if dev.index == torch.cuda.current_device():
-        check(fn(*args, stream()))
+    if dev.type != "cuda":
+        raise CvgError("cvae_gan_amd ops need device tensors")
+    if dev.index == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
     else:
         with torch.cuda.device(dev):
-            check(fn(*args, stream()))
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    if rc != 0:
+        check(rc)
 
 
 def _p(t):
@@ -396,23 +400,26 @@ def _nbytes(t):
     return 0 if t is None else t.numel() * t.element_size()
 
 
-def _scratch(ws, n, device):
+def _scratch(ws, query, d, backward, device):
     if ws is None:
+        n = int(query(C.byref(d), backward))
         return _bytes(n, device) if n else None
-    _need(ws.device == device and ws.is_contiguous(), "the workspace has to be contiguous on %s", device)
+    if ws.device != device or not ws.is_contiguous():
+        raise CvgError("the workspace has to be contiguous on %s" % device)
     return ws
 
 
+_ACT_VALUES = frozenset(ACTS.values())
+
+
 def _gn_desc(x, G, act, eps=0.0):
-    _need(x.dim() >= 2 and x.dtype in _DT, "x has to be [B, ..., C] in float32 or bfloat16")
-    B, C_ = x.shape[0], x.shape[-1]
+    shape = x.shape
+    _need(len(shape) >= 2 and x.dtype in _DT, "x has to be [B, ..., C] in float32 or bfloat16")
     hw = 1
-    for n in x.shape[1:-1]:
+    for n in shape[1:-1]:
         hw *= n
-    _need(act in ACTS.values(), "activation %r", act)
-    d = GnDesc()
-    d.dtype, d.B, d.HW, d.C, d.G, d.act, d.eps = _DT[x.dtype], B, hw, C_, int(G), act, eps
-    return d
+    _need(act in _ACT_VALUES, "activation %r", act)
+    return GnDesc(_DT[x.dtype], shape[0], hw, shape[-1], int(G), act, 0, 0, 0, 0, 0, eps)
 
 
 def gn_act_workspace(x, G, backward=False):
@@ -424,54 +431,50 @@ def gn_act_fwd(x, res, y, G, stats, gamma, beta, eps=1e-5, act=ACT_LRELU, ws=Non
     """y = act(groupnorm(x) * gamma + beta [+ res]); x, res, y [B, ..., C] channels last, stats f32 [2, B, G] (mean,
     1 / std; None: not kept), gamma / beta f32 [C]."""
     d = _gn_desc(x, G, act, eps)
-    _like("res", res, "x", x)
-    _like("y", y, "x", x)
-    for n, t in (("gamma", gamma), ("beta", beta)):
-        _like(n, t, "x", x, (d.C,), torch.float32)
-        _dense(n, t)
-    _like("stats", stats, "x", x, (2, d.B, d.G), torch.float32)
-    _dense("stats", stats)
+    dev, c = x.device, (d.C,)
+    _is("res", res, x.shape, x.dtype, dev)
+    _is("y", y, x.shape, x.dtype, dev)
+    _vec("gamma", gamma, c, dev)
+    _vec("beta", beta, c, dev)
+    _vec("stats", stats, (2, d.B, d.G), dev)
     d.x_ld, d.res_ld, d.y_ld = _pitch("x", x), _pitch("res", res), _pitch("y", y)
-    ws = _scratch(ws, 0 if ws is not None else int(lib.cvg_gn_act_workspace(C.byref(d), 0)), x.device)
-    _launch(lib.cvg_gn_act_fwd, x.device, C.byref(d), _p(x), _p(res), _p(y), _p(stats), _p(gamma), _p(beta), _p(ws), _nbytes(ws))
+    ws = _scratch(ws, lib.cvg_gn_act_workspace, d, 0, dev)
+    _launch(lib.cvg_gn_act_fwd, dev, C.byref(d), _p(x), _p(res), _p(y), _p(stats), _p(gamma), _p(beta), _p(ws), _nbytes(ws))
 
 
 def gn_act_bwd(dy, x, res, dx, dres, G, stats, gamma, beta, dgamma, dbeta, act=ACT_LRELU, ws=None):
     """Gradients of gn_act_fwd: res as in the forward call, stats from it; dres may be None."""
     d = _gn_desc(x, G, act)
+    dev, c = x.device, (d.C,)
     for n, t in (("dy", dy), ("res", res), ("dx", dx), ("dres", dres)):
-        _like(n, t, "x", x)
+        _is(n, t, x.shape, x.dtype, dev)
     for n, t in (("gamma", gamma), ("beta", beta), ("dgamma", dgamma), ("dbeta", dbeta)):
-        _like(n, t, "x", x, (d.C,), torch.float32)
-        _dense(n, t)
-    _like("stats", stats, "x", x, (2, d.B, d.G), torch.float32)
-    _dense("stats", stats)
+        _vec(n, t, c, dev)
+    _vec("stats", stats, (2, d.B, d.G), dev)
     d.x_ld, d.res_ld, d.y_ld = _pitch("x", x), _pitch("res", res), _pitch("dy", dy)
     d.dx_ld, d.dres_ld = _pitch("dx", dx), _pitch("dres", dres)
-    ws = _scratch(ws, 0 if ws is not None else int(lib.cvg_gn_act_workspace(C.byref(d), 1)), x.device)
-    _launch(lib.cvg_gn_act_bwd, x.device, C.byref(d), _p(dy), _p(x), _p(res), _p(dx), _p(dres), _p(stats), _p(gamma), _p(beta),
+    ws = _scratch(ws, lib.cvg_gn_act_workspace, d, 1, dev)
+    _launch(lib.cvg_gn_act_bwd, dev, C.byref(d), _p(dy), _p(x), _p(res), _p(dx), _p(dres), _p(stats), _p(gamma), _p(beta),
             _p(dgamma), _p(dbeta), _p(ws), _nbytes(ws))
 
 
 def _linear_desc(x, w, act):
     _need(x.dim() >= 1 and w.dim() == 2 and x.dtype in _DT, "x has to be [..., K] and w [N, K], in float32 or bfloat16")
     N, K = w.shape
-    _like("w", w, "x", x, (N, x.shape[-1]))
-    _need(act in ACTS.values(), "activation %r", act)
-    d = LinearDesc()
+    _is("w", w, (N, x.shape[-1]), x.dtype, x.device)
+    _need(act in _ACT_VALUES, "activation %r", act)
     m = 1
     for n in x.shape[:-1]:
         m *= n
-    d.dtype, d.M, d.N, d.K, d.act, d.dw_dtype, d.pre_dtype = _DT[x.dtype], m, N, K, act, F32, F32
-    d.x_ld, d.w_ld = _pitch("x", x), _pitch("w", w)
-    return d
+    return LinearDesc(_DT[x.dtype], m, N, K, act, F32, F32, _pitch("x", x), _pitch("w", w))
 
 
 def _pre(d, pre, x, shape):
     if pre is not None:
-        _need(pre.dtype in (torch.float32, x.dtype), "pre is %s", pre.dtype)
-        _like("pre", pre, "x", x, shape, pre.dtype)
+        _need(pre.dtype == torch.float32 or pre.dtype == x.dtype, "pre is %s", pre.dtype)
+        _is("pre", pre, shape, pre.dtype, x.device)
         d.pre_dtype = _DT[pre.dtype]
+        d.pre_ld = _pitch("pre", pre)
 
 
 def linear_act_workspace(x, w, act=ACT_NONE, backward=False):
@@ -484,34 +487,32 @@ def linear_act_fwd(x, w, y, bias=None, res=None, pre=None, act=ACT_NONE, ws=None
     """y = act(x @ w.T + bias) + res; x [..., K], w [N, K], y / res / pre [..., N], bias f32 [N].  pre (float32
     or x's type) receives the activation's argument for linear_act_bwd."""
     d = _linear_desc(x, w, act)
-    out = tuple(x.shape[:-1]) + (d.N,)
-    for n, t in (("y", y), ("res", res)):
-        _like(n, t, "x", x, out)
+    dev, out = x.device, x.shape[:-1] + (d.N,)
+    _is("y", y, out, x.dtype, dev)
+    _is("res", res, out, x.dtype, dev)
     _pre(d, pre, x, out)
-    _like("bias", bias, "x", x, (d.N,), torch.float32)
-    _dense("bias", bias)
-    d.y_ld, d.res_ld, d.pre_ld = _pitch("y", y), _pitch("res", res), _pitch("pre", pre)
-    ws = _scratch(ws, 0 if ws is not None else int(lib.cvg_linear_act_workspace(C.byref(d), 0)), x.device)
-    _launch(lib.cvg_linear_act_fwd, x.device, C.byref(d), _p(x), _p(w), _p(bias), _p(res), _p(y), _p(pre), _p(ws), _nbytes(ws))
+    _vec("bias", bias, (d.N,), dev)
+    d.y_ld, d.res_ld = _pitch("y", y), _pitch("res", res)
+    ws = _scratch(ws, lib.cvg_linear_act_workspace, d, 0, dev)
+    _launch(lib.cvg_linear_act_fwd, dev, C.byref(d), _p(x), _p(w), _p(bias), _p(res), _p(y), _p(pre), _p(ws), _nbytes(ws))
 
 
 def linear_act_bwd(dy, x, w, pre=None, dx=None, dw=None, dbias=None, act=ACT_NONE, ws=None):
     """Gradients of linear_act_fwd, each optional: dx like x, dw [N, K] (float32 or x's type), dbias f32 [N].  An
     activation needs the pre of the forward call; the gradient of res is dy itself."""
     d = _linear_desc(x, w, act)
-    out = tuple(x.shape[:-1]) + (d.N,)
-    _like("dy", dy, "x", x, out)
+    dev, out = x.device, x.shape[:-1] + (d.N,)
+    _is("dy", dy, out, x.dtype, dev)
     _pre(d, pre, x, out)
-    _like("dx", dx, "x", x)
+    _is("dx", dx, x.shape, x.dtype, dev)
     if dw is not None:
-        _need(dw.dtype in (torch.float32, x.dtype), "dw is %s", dw.dtype)
-        _like("dw", dw, "x", x, w.shape, dw.dtype)
+        _need(dw.dtype == torch.float32 or dw.dtype == x.dtype, "dw is %s", dw.dtype)
+        _is("dw", dw, w.shape, dw.dtype, dev)
         d.dw_dtype = _DT[dw.dtype]
-    _like("dbias", dbias, "x", x, (d.N,), torch.float32)
-    _dense("dbias", dbias)
-    d.dy_ld, d.pre_ld, d.dx_ld, d.dw_ld = _pitch("dy", dy), _pitch("pre", pre), _pitch("dx", dx), _pitch("dw", dw)
-    ws = _scratch(ws, 0 if ws is not None else int(lib.cvg_linear_act_workspace(C.byref(d), 1)), x.device)
-    _launch(lib.cvg_linear_act_bwd, x.device, C.byref(d), _p(dy), _p(x), _p(w), _p(pre), _p(dx), _p(dw), _p(dbias), _p(ws),
+    _vec("dbias", dbias, (d.N,), dev)
+    d.dy_ld, d.dx_ld, d.dw_ld = _pitch("dy", dy), _pitch("dx", dx), _pitch("dw", dw)
+    ws = _scratch(ws, lib.cvg_linear_act_workspace, d, 1, dev)
+    _launch(lib.cvg_linear_act_bwd, dev, C.byref(d), _p(dy), _p(x), _p(w), _p(pre), _p(dx), _p(dw), _p(dbias), _p(ws),
             _nbytes(ws))
 
 
@@ -519,25 +520,20 @@ def distill_topk(logits, top_val, top_idx, loss, row_loss, dlogits=None, row_wei
     """Distillation loss against a teacher's top logits, and its gradient: logits [..., V], top_val f32 / top_idx int32
     [..., top], row_loss / row_weight f32 [...], loss f32 scalar (one element); dlogits like logits (or logits itself)."""
     _need(logits.dim() >= 1 and logits.dtype in _DT, "logits have to be [..., V] in float32 or bfloat16")
-    rows = tuple(logits.shape[:-1])
     _need(top_val.dim() >= 1, "top_val has to be [..., top]")
-    d = DistillDesc()
-    d.dtype, d.V, d.top = _DT[logits.dtype], logits.shape[-1], top_val.shape[-1]
-    d.R = 1
+    rows, dev, top = logits.shape[:-1], logits.device, top_val.shape[-1]
+    r = 1
     for n in rows:
-        d.R *= n
-    _like("top_val", top_val, "logits", logits, rows + (d.top,), torch.float32)
-    _like("top_idx", top_idx, "logits", logits, rows + (d.top,), torch.int32)
-    _like("row_loss", row_loss, "logits", logits, rows, torch.float32)
-    _like("row_weight", row_weight, "logits", logits, rows, torch.float32)
-    _like("dlogits", dlogits, "logits", logits)
-    _need(loss.numel() == 1 and loss.dtype == torch.float32 and loss.device == logits.device, "loss has to be one float32 on %s",
-          logits.device)
-    _dense("row_loss", row_loss)
-    _dense("row_weight", row_weight)
-    d.logits_ld, d.dlogits_ld = _pitch("logits", logits), _pitch("dlogits", dlogits)
-    d.top_ld = _pitch("top_val", top_val)
-    _need((d.top_ld or d.top) == (_pitch("top_idx", top_idx) or d.top), "top_val and top_idx have to share their strides")
-    d.temperature, d.grad_scale = float(temperature), float(grad_scale)
-    _launch(lib.cvg_distill_topk, logits.device, C.byref(d), _p(logits), _p(top_val), _p(top_idx), _p(row_weight), _p(loss),
+        r *= n
+    _is("top_val", top_val, rows + (top,), torch.float32, dev)
+    _is("top_idx", top_idx, rows + (top,), torch.int32, dev)
+    _vec("row_loss", row_loss, rows, dev)
+    _vec("row_weight", row_weight, rows, dev)
+    _is("dlogits", dlogits, logits.shape, logits.dtype, dev)
+    _need(loss.numel() == 1 and loss.dtype == torch.float32 and loss.device == dev, "loss has to be one float32 on %s", dev)
+    top_ld = _pitch("top_val", top_val)
+    _need((top_ld or top) == (_pitch("top_idx", top_idx) or top), "top_val and top_idx have to share their strides")
+    d = DistillDesc(_DT[logits.dtype], r, logits.shape[-1], top, _pitch("logits", logits), _pitch("dlogits", dlogits), top_ld,
+                    float(temperature), float(grad_scale))
+    _launch(lib.cvg_distill_topk, dev, C.byref(d), _p(logits), _p(top_val), _p(top_idx), _p(row_weight), _p(loss),
             _p(row_loss), _p(dlogits))
