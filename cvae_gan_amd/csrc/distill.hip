@@ -6,8 +6,11 @@
 // TPR threads own a row (a wave, 256 threads or 1024) and hold it in registers, R vectors of 8 each: every vector goes
 // into a running (maximum, sum of exponentials) as it arrives, so the sum is taken while the rest of the row is still on
 // its way, and the gradient is computed from the same registers: the logits are read once, the gradient is written once.
+// A workgroup walks over rows, and as soon as a vector's gradient is stored its registers take the same vector of the
+// next row: loads, arithmetic and stores of two rows overlap although one row fills the register file.
 // Rows that do not fit (131072 bf16 or 65536 f32 classes) are read twice, the second time mostly from the 256 MB cache.
-// The k classes of the teacher are written after a barrier, over the q the row pass left there.
+// The k teacher entries sit in a hash table in LDS, keyed by the vector of 8 their class falls into; whoever computes
+// that vector's gradient subtracts them and takes their part of the loss, so nothing is gathered or written twice.
 #include "rowops.h"
 
 namespace {
@@ -40,22 +43,21 @@ template <int TPR> __device__ __forceinline__ float row_sum(float v, float* sh) 
 }
 
 #define LOG2E 1.4426950408889634f
-#define LN2 0.6931471805599453f
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// Running (maximum, sum of 2^(k (v - maximum))).  The maximum starts at the lowest finite value, so that a row may begin
-// with -inf; a NaN or +inf reaches the sum.
+// Running (maximum, sum of 2^(k (v - maximum))).  The maximum is subtracted before k is multiplied in: k times the lowest
+// values of a type overflows, and a row that is masked throughout is uniform.  It starts at the lowest finite value, so
+// that a row may begin with -inf; a NaN or +inf reaches the sum.
 struct Running {
     float m, s;
     __device__ __forceinline__ void add(const float (&v)[8], float k) {
-        float n = m;
+        const float before = m;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) n = fmaxf(n, v[j]);
+        for (int j = 0; j < 8; ++j) m = v[j] > m ? v[j] : m;
         float t = 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) t += exp2_((v[j] - n) * k);
-        s = s * exp2_((m - n) * k) + t;
-        m = n;
+        for (int j = 0; j < 8; ++j) t += exp2_((v[j] - m) * k);
+        s = fmaf(s, exp2_((before - m) * k), t);
     }
     __device__ __forceinline__ void join(float m2, float s2, float k) {
         const float n = fmaxf(m, m2);
@@ -63,17 +65,6 @@ struct Running {
         m = n;
     }
 };
-template <int TPR> __device__ __forceinline__ void row_join(Running& r, float k, float* sh) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) r.join(__shfl_xor(r.m, o, 64), __shfl_xor(r.s, o, 64), k);
-    if (TPR == 64) return;
-    if ((threadIdx.x & 63) == 0) { sh[threadIdx.x >> 6] = r.m; sh[16 + (threadIdx.x >> 6)] = r.s; }
-    __syncthreads();
-    r.m = sh[0];
-    r.s = sh[16];
-#pragma unroll
-    for (int i = 1; i < TPR / 64; ++i) r.join(sh[i], sh[16 + i], k);
-}
 
 // The row as vectors of 8 elements on 16-byte borders: vector i covers elements [8 i - sh, 8 i - sh + 8), where sh is
 // how far behind a border the row starts; the first and the last vector may hang over the row and go element by element.
@@ -98,159 +89,276 @@ template <typename T> __device__ __forceinline__ void vec_store(T* base, int sh,
 }
 
 template <typename T> __device__ __forceinline__ bool vec_inside(int sh, int V, int i) { return i * 8 - sh >= 0 && i * 8 - sh + 8 <= V; }
-
-// R = 0: the row is read from memory twice
-template <typename T, int TPR, int R>
-__global__ void __launch_bounds__(TPR == 64 ? 256 : TPR) distill_row(const DistillArgs a) {
-    constexpr int ROWS = TPR == 64 ? 4 : 1;
-    __shared__ float sh[32];
-    extern __shared__ float dyn[];                        // [ROWS][top] p, then [ROWS][top] class indices
-    const int sub = ROWS == 1 ? 0 : threadIdx.x >> 6, tid = ROWS == 1 ? threadIdx.x : threadIdx.x & 63, lane = threadIdx.x & 63;
-    const int r = blockIdx.x * ROWS + sub;
-    if (ROWS > 1 && r >= a.R) return;                     // (whole waves; the wave form has no barrier)
-    float* tp = dyn + sub * a.top;
-    int32_t* ti = (int32_t*)(dyn + ROWS * a.top) + sub * a.top;
-    const T* row = (const T*)a.logits + (size_t)r * a.ld;
-    T* out = a.dlogits ? (T*)a.dlogits + (size_t)r * a.dld : nullptr;
-    const int off = (int)(((uintptr_t)row & 15) / sizeof(T));
-    const bool whole = out && ((((uintptr_t)out) ^ (uintptr_t)row) & 15) == 0;
-    const int nvec = (off + a.V + 7) / 8;
-    const float k = a.inv_t * LOG2E;
-
-    Raw8<T> x[R > 0 ? R : 1];
-    if constexpr (R > 0) {                                // everything is requested before anything is waited for
-#pragma unroll
-        for (int u = 0; u < R; ++u) {
-            const int i = tid + u * TPR;
-            if (i < nvec && vec_inside<T>(off, a.V, i)) raw_load(x[u], row + i * 8 - off);
-            else {
-                float v[8];
-                vec_load<T>(row, off, a.V, i, v);
-                raw_pack(x[u], v);
-            }
-        }
-    }
-    // The teacher: every wave takes the maximum and the sum over all entries, so no wave waits for another.
-    const float w = a.row_weight ? a.row_weight[r] : 1.f;
-    const float* val = a.top_val + (size_t)r * a.tld;
-    const int32_t* idx = a.top_idx + (size_t)r * a.tld;
-    auto entry = [&](int j, int& i) {
-        i = idx[j];
-        const float v = val[j] * a.inv_t;
-        if (i < 0 || i >= a.V || v == -INFINITY) i = -1;
-        return i < 0 ? -INFINITY : v;
-    };
-    float tmax = -INFINITY, ps = 0.f, v0 = -INFINITY;
-    int i0 = -1;
-    if (lane < a.top) v0 = tmax = entry(lane, i0);        // (the first 64 entries are read once)
-    for (int j = lane + 64; j < a.top; j += 64) { int i; tmax = fmaxf(tmax, entry(j, i)); }
-    tmax = wave_max(tmax);
-    if (i0 >= 0) ps = expf(v0 - tmax);
-    for (int j = lane + 64; j < a.top; j += 64) {
-        int i;
-        const float v = entry(j, i);
-        if (i >= 0) ps += expf(v - tmax);
-    }
-    ps = wave_sum(ps);                                    // 0: no entry at all (the largest adds 1, a NaN stays)
-    if (w == 0.f || ps == 0.f) {                          // (the same for every thread of the row)
-        if (tid == 0) a.row_loss[r] = 0.f;
-        if (out) {
-            const float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            for (int i = tid; i < nvec; i += TPR) vec_store<T>(out, off, a.V, i, whole, z);
-        }
-        return;
-    }
-
-    Running run{-3.402823466e38f, 0.f};
-    if constexpr (R > 0) {
-#pragma unroll
-        for (int u = 0; u < R; ++u) {
-            if (tid + u * TPR < nvec) {
-                float v[8];
-                raw_f32(x[u], v);
-                run.add(v, k);
-            }
-        }
+template <typename T> __device__ __forceinline__ void vec_raw(Raw8<T>& x, const T* row, int sh, int V, int i) {
+    if (vec_inside<T>(sh, V, i)) {
+        raw_load(x, row + i * 8 - sh);
     } else {
-        for (int i = tid; i < nvec; i += TPR) {
-            float v[8];
-            vec_load<T>(row, off, a.V, i, v);
-            run.add(v, k);
-        }
-    }
-    row_join<TPR>(run, k, sh);
-    const float m = run.m, logz = logf(run.s), inv_z = 1.f / run.s, logp0 = logf(ps);
-    // loss terms; p, the class and q at the class are kept for the gradient (q before the row is overwritten: dlogits may
-    // be logits)
-    float l = 0.f, qj[MAX_TOP / TPR > 0 ? MAX_TOP / TPR : 1];
-#pragma unroll
-    for (int u = 0; u < (MAX_TOP + TPR - 1) / TPR; ++u) {
-        const int j = tid + u * TPR;
-        if (j >= a.top) break;
-        int i = i0;
-        const float v = TPR == 64 && u == 0 ? v0 : entry(j, i), lp = v - tmax - logp0, p = i < 0 ? 0.f : expf(v - tmax) / ps;
-        const float z = i < 0 ? 0.f : (to_f32(row[i]) - m) * a.inv_t;
-        if (i >= 0 && (p > 0.f || p != p)) l += p * (lp - (z - logz));
-        qj[u] = i < 0 ? 0.f : expf(z) * inv_z;
-        tp[j] = p;
-        ti[j] = i;
-    }
-    l = row_sum<TPR>(l, sh);                              // (its barriers also publish tp and ti, and end the reads of the row)
-    if (tid == 0) a.row_loss[r] = w * a.temp * a.temp * l;
-    if (!out) return;
-    const float c = a.scale * w * a.temp, cz = c * inv_z;
-    if constexpr (R > 0) {
-#pragma unroll
-        for (int u = 0; u < R; ++u) {
-            const int i = tid + u * TPR;
-            if (i < nvec) {
-                float v[8];
-                raw_f32(x[u], v);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = cz * exp2_((v[j] - m) * k);
-                vec_store<T>(out, off, a.V, i, whole, v);
-            }
-        }
-    } else {
-        for (int i = tid; i < nvec; i += TPR) {
-            float v[8];
-            vec_load<T>(row, off, a.V, i, v);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = cz * exp2_((v[j] - m) * k);
-            vec_store<T>(out, off, a.V, i, whole, v);
-        }
-    }
-    // the row's stores are acknowledged before the teacher's classes are written over them
-    if (TPR == 64) __threadfence_block(); else __syncthreads();
-#pragma unroll
-    for (int u = 0; u < (MAX_TOP + TPR - 1) / TPR; ++u) {
-        const int j = tid + u * TPR;
-        if (j >= a.top) break;
-        if (ti[j] < 0) continue;
-        // an index that appears more than once: its first entry writes the sum
-        float p = 0.f;
-        bool first = true;
-        for (int e = 0; e < a.top; ++e)
-            if (ti[e] == ti[j]) { first &= e >= j; p += tp[e]; }
-        if (first) out[ti[j]] = from_f32<T>(c * (qj[u] - p));
+        float v[8];
+        vec_load<T>(row, sh, V, i, v);
+        raw_pack(x, v);
     }
 }
 
+// only LDS is exchanged behind these barriers: global loads and stores stay in flight
+template <int TPR> __device__ __forceinline__ void row_barrier() {
+    if (TPR == 64) {                                      // (a wave's LDS accesses complete in order)
+        asm volatile("" : : : "memory");
+        return;
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" : : : "memory");
+}
+
+// EVEN: every row starts on a 16-byte border and is a whole number of vectors.  R = 0: the row is read from memory twice.
+template <typename T, int TPR, int R, bool EVEN>
+__global__ void __launch_bounds__(TPR == 64 ? 256 : TPR, 4) distill_row(const DistillArgs a) {
+    constexpr int ROWS = TPR == 64 ? 4 : 1, HASH = TPR == 64 ? 256 : 2048;
+    __shared__ float sh[64];
+    __shared__ int32_t heads[ROWS][HASH];
+    extern __shared__ float dyn[];                        // [ROWS][4][top]: value, class, p (of all entries of the class), next
+    const int sub = ROWS == 1 ? 0 : threadIdx.x >> 6, tid = ROWS == 1 ? threadIdx.x : threadIdx.x & 63, lane = threadIdx.x & 63;
+    int r = blockIdx.x * ROWS + sub;
+    if (r >= a.R) return;                                 // (whole waves; only the wave form can have idle ones)
+    float* tv = dyn + sub * 4 * a.top;
+    int32_t* ti = (int32_t*)(tv + a.top);
+    float* tp = tv + 2 * a.top;
+    int32_t* next = (int32_t*)(tv + 3 * a.top);
+    int32_t* head = heads[sub];
+    const float k = a.inv_t * LOG2E;
+    const int stride = gridDim.x * ROWS;
+    constexpr uint32_t VB = 8 * sizeof(T);               // bytes of a vector
+
+    const T* row = (const T*)a.logits + (size_t)r * a.ld;
+    int off = EVEN ? 0 : (int)(((uintptr_t)row & 15) / sizeof(T)), nvec = (off + a.V + 7) / 8;
+    // this thread's first teacher entry (the only one where there are as many threads as entries) travels a row ahead
+    const int my = min(tid, a.top - 1);
+    float ev = a.top_val[(size_t)r * a.tld + my];
+    int32_t ei = a.top_idx[(size_t)r * a.tld + my];
+    float w = a.row_weight ? a.row_weight[r] : 1.f;
+    // Loads and stores of the EVEN form are unconditional (lanes behind the row repeat its last vector, and store the same
+    // values there): under a branch the compiler could not tell how many are in flight and would wait for all of them.
+    Raw8<T> x[R > 0 ? R : 1];
+    if constexpr (R > 0) {
+#pragma unroll
+        for (int u = 0; u < R; ++u) {
+            const int i = tid + u * TPR;
+            if constexpr (EVEN) raw_load(x[u], (const T*)((const char*)row + (uint32_t)min(i, nvec - 1) * VB));
+            else if (i < nvec) vec_raw<T>(x[u], row, off, a.V, i);
+        }
+    }
+
+    for (;;) {
+        T* out = a.dlogits ? (T*)a.dlogits + (size_t)r * a.dld : nullptr;
+        const bool whole = EVEN || (out && ((((uintptr_t)out) ^ (uintptr_t)row) & 15) == 0);
+        // ---- the teacher: entries into LDS, their maximum and sum, chains by vector
+        float v0 = ev * a.inv_t;
+        int c0 = ei;
+        if (c0 < 0 || c0 >= a.V || v0 == -INFINITY) { c0 = -1; v0 = -INFINITY; }
+        float s0 = to_f32(row[max(c0, 0)]);               // the student's logit at this thread's first class
+        if (tid < a.top) { tv[tid] = v0; ti[tid] = c0; }
+        for (int j = tid + TPR; j < a.top; j += TPR) {
+            const float v = a.top_val[(size_t)r * a.tld + j] * a.inv_t;
+            const int c = a.top_idx[(size_t)r * a.tld + j];
+            const bool in = c >= 0 && c < a.V && v != -INFINITY;
+            tv[j] = in ? v : -INFINITY;
+            ti[j] = in ? c : -1;
+        }
+        for (int i = tid; i < HASH; i += TPR) head[i] = -1;
+        row_barrier<TPR>();
+        float tmax = -INFINITY, ps = 0.f;                 // (every wave takes them over all entries)
+        for (int j = lane; j < a.top; j += 64) tmax = fmaxf(tmax, tv[j]);
+        tmax = wave_max(tmax);
+        for (int j = lane; j < a.top; j += 64)
+            if (ti[j] >= 0) ps += expf(tv[j] - tmax);
+        ps = wave_sum(ps);                                // 0: no entry at all (the largest adds 1, a NaN stays)
+        const bool dead = w == 0.f || ps == 0.f;
+        const float logp0 = logf(ps) + tmax;
+        if (!dead)
+            for (int j = tid; j < a.top; j += TPR) {
+                const int c = ti[j];
+                if (c < 0 || expf(tv[j] - logp0) == 0.f) { next[j] = -2; continue; }      // (absent, or nothing to add)
+                next[j] = atomicExch(&head[((c + off) >> 3) & (HASH - 1)], j);
+            }
+        row_barrier<TPR>();
+        if (!dead)
+            for (int j = tid; j < a.top; j += TPR) {
+                // p of the class: where entries name it twice the first stands for all, added in their order, whatever the
+                // order in which they were chained
+                const int c = ti[j];
+                float p = 0.f;
+                if (next[j] != -2) {
+                    for (int last = -1;;) {
+                        int e = MAX_TOP;
+                        for (int q = head[((c + off) >> 3) & (HASH - 1)]; q >= 0; q = next[q])
+                            if (q > last && q < e && ti[q] == c) e = q;
+                        if (last < 0 && e != j) break;    // (not the first)
+                        if (e == MAX_TOP) break;
+                        p += expf(tv[e] - logp0);
+                        last = e;
+                    }
+                }
+                tp[j] = p;
+            }
+        // ---- maximum and sum
+        Running run{-3.402823466e38f, 0.f};
+        if constexpr (R > 0) {
+#pragma unroll
+            for (int u = 0; u < R; ++u) {
+                if (tid + u * TPR < nvec) {
+                    float v[8];
+                    pin(x[u]);
+                    raw_f32(x[u], v);
+                    run.add(v, k);
+                }
+            }
+        } else {
+            for (int i = tid; i < nvec; i += TPR) {
+                float v[8];
+                vec_load<T>(row, off, a.V, i, v);
+                run.add(v, k);
+            }
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) run.join(__shfl_xor(run.m, o, 64), __shfl_xor(run.s, o, 64), k);
+        asm volatile("" : "+v"(s0));                      // (arrived: behind the barrier the row may be overwritten)
+        if (TPR > 64) {
+            if (lane == 0) { sh[tid >> 6] = run.m; sh[16 + (tid >> 6)] = run.s; }
+            row_barrier<TPR>();                           // (publishes tp too)
+            run.m = sh[0];
+            run.s = sh[16];
+#pragma unroll
+            for (int i = 1; i < TPR / 64; ++i) run.join(sh[i], sh[16 + i], k);
+        }
+        const float m = run.m, inv_z = 1.f / run.s, c = a.scale * w * a.temp, cz = c * inv_z;
+        // ---- the loss: T^2 p (log p - log q) as T p (T log p - ((s - maximum) - T log z)), which does not divide a masked
+        // logit by a temperature below one
+        float l = 0.f;
+        if (!dead) {
+            const float tz = a.temp * logf(run.s), wt = w * a.temp;
+            for (int j = tid; j < a.top; j += TPR) {
+                if (next[j] == -2) continue;
+                const float lp = tv[j] - logp0, v = j == tid ? s0 : to_f32(row[ti[j]]);
+                l += wt * expf(lp) * (a.temp * lp - ((v - m) - tz));
+            }
+        }
+        // ---- the gradient; the next row moves in
+        const int rn = r + stride;
+        const bool more = rn < a.R;
+        const T* row_n = more ? (const T*)a.logits + (size_t)rn * a.ld : row;
+        const int off_n = EVEN ? 0 : (int)(((uintptr_t)row_n & 15) / sizeof(T)), nvec_n = (off_n + a.V + 7) / 8;
+        const int r_next = more ? rn : r;
+        ev = a.top_val[(size_t)r_next * a.tld + my];
+        ei = a.top_idx[(size_t)r_next * a.tld + my];
+        w = a.row_weight ? a.row_weight[r_next] : 1.f;
+        if (TPR > 64 && a.top > TPR) {                    // (the loads of the loop above have arrived in every wave)
+            asm volatile("" : "+v"(l));
+            row_barrier<TPR>();
+        }
+        auto gradient = [&](float (&v)[8], int i) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = cz * exp2_((v[j] - m) * k);
+            for (int q = head[i & (HASH - 1)]; q >= 0; q = next[q]) {
+                const int at = ti[q] + off - 8 * i;
+                const float p = c * tp[q];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] -= j == at ? p : 0.f;
+            }
+        };
+        // (a fresh copy of tid per row: what depends on it is recomputed where it is used instead of being kept in R
+        // registers across rows)
+        int t = tid;
+        asm volatile("" : "+v"(t));
+        const int last_n = more ? nvec_n - 1 : 0;         // (no next row: one line, loaded and never used)
+        if constexpr (R > 0 && EVEN) {
+            // one path for every row (two would meet with the loads in different registers, and wait for them to move)
+#pragma unroll
+            for (int u = 0; u < R; ++u) {
+                const int i = min(t + u * TPR, nvec - 1);
+                float v[8];
+                pin(x[u]);
+                if (dead) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[j] = 0.f;
+                } else {
+                    raw_f32(x[u], v);
+                    gradient(v, i);
+                }
+                if (R > 4 || out) store8<T>((T*)((char*)out + (uint32_t)i * VB), v);       // (R > 4 is launched with an output)
+                raw_load(x[u], (const T*)((const char*)row_n + (uint32_t)min(t + u * TPR, last_n) * VB));
+            }
+        } else if constexpr (R > 0) {
+#pragma unroll
+            for (int u = 0; u < R; ++u) {
+                const int i = t + u * TPR;
+                if (out && i < nvec) {
+                    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                    pin(x[u]);
+                    if (!dead) {
+                        raw_f32(x[u], v);
+                        gradient(v, i);
+                    }
+                    vec_store<T>(out, off, a.V, i, whole, v);
+                }
+                if (more && i < nvec_n) vec_raw<T>(x[u], row_n, off_n, a.V, i);
+            }
+        } else if (out) {
+            for (int i = tid; i < nvec; i += TPR) {
+                float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                if (!dead) {
+                    vec_load<T>(row, off, a.V, i, v);
+                    gradient(v, i);
+                }
+                vec_store<T>(out, off, a.V, i, whole, v);
+            }
+        }
+        l = wave_sum(l);
+        if (TPR > 64) {
+            if (lane == 0) sh[32 + (tid >> 6)] = l;
+            row_barrier<TPR>();                           // (and the table may be cleared)
+            l = 0.f;
+#pragma unroll
+            for (int i = 0; i < TPR / 64; ++i) l += sh[32 + i];
+        }
+        if (tid == 0) a.row_loss[r] = l;
+        if (!more) return;
+        r = rn;
+        row = row_n;
+        off = off_n;
+        nvec = nvec_n;
+    }
+}
+
+template <typename T, int TPR, int R>
+void launch_as(const DistillArgs& a, bool even, int per_cu, hipStream_t st) {
+    constexpr int ROWS = TPR == 64 ? 4 : 1;
+    const size_t lds = (size_t)a.top * 16 * ROWS;
+    // as many workgroups as the chip holds at once; each walks over its share of the rows
+    const int blocks = min(ceil_div(a.R, ROWS), 256 * per_cu);
+    if (even) distill_row<T, TPR, R, true><<<blocks, TPR == 64 ? 256 : TPR, lds, st>>>(a);
+    else distill_row<T, TPR, R, false><<<blocks, TPR == 64 ? 256 : TPR, lds, st>>>(a);
+}
 template <typename T>
 void launch(const DistillArgs& a, hipStream_t st) {
-    // (rows that do not all start on a 16-byte border may need one vector more)
-    const bool even = aligned16(a.logits) && a.ld * sizeof(T) % 16 == 0;
-    const int nvec = (a.V + 7) / 8 + (even ? 0 : 1);
-    const size_t lds = (size_t)a.top * 8;
     constexpr bool B = sizeof(T) == 2;
-    // a wave per row while 8 vectors per lane hold it, 256 threads for mid-sized rows, otherwise a workgroup of 1024
-    if (nvec <= 64) distill_row<T, 64, 1><<<ceil_div(a.R, 4), 256, lds * 4, st>>>(a);
-    else if (nvec <= 256) distill_row<T, 64, 4><<<ceil_div(a.R, 4), 256, lds * 4, st>>>(a);
-    else if (nvec <= 1024) distill_row<T, 256, 4><<<a.R, 256, lds, st>>>(a);
-    else if (nvec <= 4096) distill_row<T, 1024, 4><<<a.R, 1024, lds, st>>>(a);
-    else if (nvec <= 8192) distill_row<T, 1024, 8><<<a.R, 1024, lds, st>>>(a);
-    else if (B && nvec <= 16384) distill_row<T, 1024, B ? 16 : 8><<<a.R, 1024, lds, st>>>(a);
-    else distill_row<T, 1024, 0><<<a.R, 1024, lds, st>>>(a);
+    // (rows that do not all start on a 16-byte border may need one vector more)
+    const bool aligned = aligned16(a.logits) && a.ld * sizeof(T) % 16 == 0;
+    const bool even = aligned && a.V % 8 == 0 && (!a.dlogits || (aligned16(a.dlogits) && a.dld * sizeof(T) % 16 == 0));
+    const int nvec = (a.V + 7) / 8 + (aligned ? 0 : 1);
+    // A wave per row while 4 vectors per lane hold it; then as many threads as hold the row in 64 registers each, so that
+    // a CU's registers are full of rows (four, two, one) at every size.
+    constexpr int F = B ? 1 : 2;                          // (an f32 vector takes twice the registers)
+    if (nvec <= 64) launch_as<T, 64, 1>(a, even, 8, st);
+    else if (nvec <= 256) launch_as<T, 64, 4>(a, even, 4, st);
+    else if (nvec <= 1024) launch_as<T, 256, 4>(a, even, 4, st);
+    else if (!a.dlogits) launch_as<T, 1024, 0>(a, even, 2, st);        // (without a gradient the row is read once there too)
+    else if (nvec * F <= 256 * 12) launch_as<T, 256, 12 / F>(a, even, 4, st);
+    else if (nvec * F <= 256 * 16) launch_as<T, 256, 16 / F>(a, even, 4, st);
+    else if (nvec * F <= 512 * 12) launch_as<T, 512, 12 / F>(a, even, 2, st);
+    else if (nvec * F <= 512 * 16) launch_as<T, 512, 16 / F>(a, even, 2, st);
+    else if (nvec * F <= 1024 * 12) launch_as<T, 1024, 12 / F>(a, even, 1, st);
+    else if (nvec * F <= 1024 * 16) launch_as<T, 1024, 16 / F>(a, even, 1, st);
+    else launch_as<T, 1024, 0>(a, even, 2, st);
 }
 
 __global__ void __launch_bounds__(1024) distill_total(const float* __restrict__ rows, int R, float* loss) {

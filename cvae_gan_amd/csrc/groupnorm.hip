@@ -163,10 +163,6 @@ __device__ __forceinline__ void chunk_groups(const GnArgs& a, const Place& p, in
     for (int j = 0; j < 8; ++j) gi[j] = p.live ? fdiv(p.chunk * 8 + j, a.cg) : 0;
 }
 
-// (keeps the unpacking of a row where it is written: hoisted, it would wait for every row at once)
-__device__ __forceinline__ void pin(Raw8<bf16>& r) { asm volatile("" : "+v"(r.a)); }
-__device__ __forceinline__ void pin(Raw8<float>& r) { asm volatile("" : "+v"(r.a), "+v"(r.b)); }
-
 // pre = x (gamma rstd) + (beta - mean gamma rstd) (+ res) in both passes, one fma: LeakyReLU takes the same sign twice.
 // Folding the mean into the constant costs an error of u |mean| gamma rstd, what the rounding of the mean itself costs.
 template <typename T, int ACT>

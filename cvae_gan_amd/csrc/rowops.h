@@ -94,3 +94,6 @@ __device__ __forceinline__ void raw_pack(Raw8<float>& r, const float (&v)[8]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) { r.a[i] = __float_as_uint(v[i]); r.b[i] = __float_as_uint(v[4 + i]); }
 }
+// keeps the unpacking of registers where it is written: hoisted above a branch, it would wait for every load at once
+__device__ __forceinline__ void pin(Raw8<bf16>& r) { asm volatile("" : "+v"(r.a)); }
+__device__ __forceinline__ void pin(Raw8<float>& r) { asm volatile("" : "+v"(r.a), "+v"(r.b)); }

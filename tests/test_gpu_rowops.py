@@ -32,6 +32,8 @@ def ops():
 def within(got, ref, slack, what):
     assert got.shape == ref.shape, (what, got.shape, ref.shape)
     g = got.double()
+    # a value beyond the largest finite one of the output's type rounds to infinity
+    ref = torch.where(ref.abs() > torch.finfo(got.dtype).max, ref.sign() * float("inf"), ref)
     assert torch.equal(torch.isfinite(g), torch.isfinite(ref)), what + ": non-finite values differ"
     fin = torch.isfinite(ref)
     tol = HALF[got.dtype] * ref.abs() + slack + 1e-37
@@ -428,6 +430,9 @@ def test_distill_absent_entries_masks_and_duplicates(ops, dtype, V):
     logits[7, keep[: len(keep) // 2]] = lowest          # masked classes of the student
     logits[7, keep[len(keep) // 2: -1]] = float("-inf")
     distill_check(ops, logits, tv, ti, w, 2.0, 1.0, "mixed")
+    masked = torch.full_like(logits, lowest)            # masked throughout: uniform
+    masked[1::2, V // 2] = 1.0                          # ... or but for one class
+    distill_check(ops, masked, tv, ti, w, 0.5, 1.0, "masked")
     # a masked class that the teacher wants: the loss is infinite, the gradient is not
     l2 = logits.clone()
     l2[7, other[0]] = float("-inf")
