@@ -99,15 +99,12 @@ template <typename T> __device__ __forceinline__ void vec_raw(Raw8<T>& x, const 
     }
 }
 
-// only LDS is exchanged behind these barriers: global loads and stores stay in flight
 template <int TPR> __device__ __forceinline__ void row_barrier() {
     if (TPR == 64) {                                      // (a wave's LDS accesses complete in order)
         asm volatile("" : : : "memory");
         return;
     }
-    asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" : : : "memory");
+    lds_barrier();
 }
 
 // EVEN: every row starts on a 16-byte border and is a whole number of vectors.  R = 0: the row is read from memory twice.
@@ -364,6 +361,7 @@ void launch(const DistillArgs& a, hipStream_t st) {
 __global__ void __launch_bounds__(1024) distill_total(const float* __restrict__ rows, int R, float* loss) {
     __shared__ float sh[16];
     float s = 0.f;
+#pragma unroll 8
     for (int i = threadIdx.x; i < R; i += 1024) s += rows[i];
     s = row_sum<1024>(s, sh);
     if (threadIdx.x == 0) *loss = s;

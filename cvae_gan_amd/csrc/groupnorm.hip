@@ -89,7 +89,7 @@ __device__ __forceinline__ void column_parts(const GnArgs& a, const Place& p, fl
         for (int o = a.nv; o < 8; o <<= 1)
 #pragma unroll
             for (int n = 0; n < N; ++n) v[n][0] += __shfl_xor(v[n][0], o, 64);
-        __syncthreads();             // the last readers of sm are done
+        lds_barrier();               // the last readers of sm are done
         if ((lane & 7) < a.nv)
 #pragma unroll
             for (int n = 0; n < N; ++n) sm[(n * a.ent + wave) * width + (lane & 7) * 8 + (h32 ? 4 : 0) + (h16 ? 2 : 0) + (h8 ? 1 : 0)] = v[n][0];
@@ -105,7 +105,7 @@ __device__ __forceinline__ void column_parts(const GnArgs& a, const Place& p, fl
             e = wave;
             writes = lane < a.nv;
         }
-        __syncthreads();
+        lds_barrier();
         if (writes)
 #pragma unroll
             for (int n = 0; n < N; ++n)
@@ -113,7 +113,7 @@ __device__ __forceinline__ void column_parts(const GnArgs& a, const Place& p, fl
                 for (int j = 0; j < 8; j += 4)
                     *(f32x4*)&sm[(n * a.ent + e) * width + p.chunk * 8 + j] = f32x4{v[n][j], v[n][j + 1], v[n][j + 2], v[n][j + 3]};
     }
-    __syncthreads();
+    lds_barrier();
 }
 // adds the entries: afterwards sm[n][0][c] holds the sum of channel c
 template <int N>
@@ -127,13 +127,13 @@ __device__ __forceinline__ void column_totals(const GnArgs& a, float* sm) {
         for (int i = 0; i < a.ent; ++i) s += q[i * width];
         q[0] = s;                    // only this thread touches column c
     }
-    __syncthreads();
+    lds_barrier();
 }
 
-// sums[n][g] = sum over the channels of group g and the first `ent` entries of w[c] * sm[n][entry][c] (w = 1 where null):
-// a.seg lanes per group
-template <int N>
-__device__ __forceinline__ void group_sums(const GnArgs& a, const Place& p, const float* sm, const float* w, int ent, float (*sums)[GN_MAX_GROUPS]) {
+// sums[n][g] = sum over the channels of group g and the first `ent` entries of w[c] * sm[n][entry][c] (w = 1 where null),
+// through f: a.seg lanes per group
+template <int N, typename F>
+__device__ __forceinline__ void group_sums(const GnArgs& a, const Place& p, const float* sm, const float* w, int ent, float (*sums)[GN_MAX_GROUPS], F f) {
     const int cg = a.cg.d, width = a.nv * 8, lane = threadIdx.x & 63, seg = a.seg, per = 64 / seg;
     const int n_items = ent * cg;
     for (int base = (threadIdx.x >> 6) * per; base < p.ngr; base += (blockDim.x >> 6) * per) {
@@ -151,10 +151,10 @@ __device__ __forceinline__ void group_sums(const GnArgs& a, const Place& p, cons
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             for (int o = seg >> 1; o > 0; o >>= 1) s[n] += __shfl_xor(s[n], o, 64);
-            if (g < p.ngr && (lane & (seg - 1)) == 0) sums[n][g] = s[n];
+            if (g < p.ngr && (lane & (seg - 1)) == 0) sums[n][g] = f(s[n]);
         }
     }
-    __syncthreads();
+    lds_barrier();
 }
 
 // per-channel constants of a thread's chunk
@@ -206,10 +206,11 @@ __global__ void __launch_bounds__(MAXT, WAVES) gn_fwd_tile(const GnArgs a) {
         }
     }
     column_parts<1>(a, p, acc, sm);
-    group_sums<1>(a, p, sm, nullptr, a.ent, sums);
     const float inv_n = 1.f / ((float)rows * (float)a.cg.d);
+    group_sums<1>(a, p, sm, nullptr, a.ent, sums, [&](float s) { return s * inv_n; });
 #pragma unroll
-    for (int j = 0; j < 8; ++j) { mean[j] = sums[0][gi[j]] * inv_n; acc[0][j] = 0.f; }
+    for (int j = 0; j < 8; ++j) { mean[j] = sums[0][gi[j]]; acc[0][j] = 0.f; }
+    pin(mean);
 #pragma unroll
     for (int i = 0; i < R; ++i) {
         if (p.ty + i * a.rpp < mine) {
@@ -221,11 +222,12 @@ __global__ void __launch_bounds__(MAXT, WAVES) gn_fwd_tile(const GnArgs a) {
         }
     }
     column_parts<1>(a, p, acc, sm);
-    group_sums<1>(a, p, sm, nullptr, a.ent, sums + 1);
+    // M2 of a tile, or 1 / std of the whole group
+    group_sums<1>(a, p, sm, nullptr, a.ent, sums + 1, [&](float s) { return a.tiles > 1 ? s : 1.f / sqrtf(s * inv_n + a.eps); });
     if (a.tiles > 1) {
         for (int g = threadIdx.x; g < p.ngr; g += blockDim.x) {
             float* o = a.part + (((size_t)p.b * a.G + p.g0 + g) * a.tiles + p.tile) * 2;
-            o[0] = sums[0][g] * inv_n;
+            o[0] = sums[0][g];
             o[1] = sums[1][g];
         }
         return;
@@ -233,13 +235,13 @@ __global__ void __launch_bounds__(MAXT, WAVES) gn_fwd_tile(const GnArgs a) {
     if (a.stats)
         for (int g = threadIdx.x; g < p.ngr; g += blockDim.x) {
             const size_t o = (size_t)p.b * a.G + p.g0 + g;
-            a.stats[o] = sums[0][g] * inv_n;
-            a.stats[(size_t)a.B * a.G + o] = 1.f / sqrtf(sums[1][g] * inv_n + a.eps);
+            a.stats[o] = sums[0][g];
+            a.stats[(size_t)a.B * a.G + o] = sums[1][g];
         }
     float sc[8], sh[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        sc[j] = ga[j] * (1.f / sqrtf(sums[1][gi[j]] * inv_n + a.eps));
+        sc[j] = ga[j] * sums[1][gi[j]];
         sh[j] = fmaf(-mean[j], sc[j], be[j]);
     }
     const T* rp = (const T*)a.res + row0 * a.res_ld + c;
@@ -260,7 +262,7 @@ __global__ void __launch_bounds__(MAXT, WAVES) gn_fwd_tile(const GnArgs a) {
 
 // Second kernel of the tiled form: every workgroup merges its sample's (mean, M2) partials, then applies.
 template <typename T, int ACT>
-__global__ void __launch_bounds__(1024) gn_fwd_apply(const GnArgs a) {
+__global__ void __launch_bounds__(512) gn_fwd_apply(const GnArgs a) {
     __shared__ float mu[GN_MAX_GROUPS], rs[GN_MAX_GROUPS];
     const Place p = gn_place(a);
     const int lane = threadIdx.x & 63, cg = a.cg.d;
@@ -395,15 +397,15 @@ __global__ void __launch_bounds__(MAXT, WAVES) gn_bwd_tile(const GnArgs a) {
         o[a.C + t] = sm[(size_t)a.ent * width + t];
     }
     if (a.tiles > 1) return;
-    group_sums<2>(a, p, sm, a.gamma, 1, sums);
     const float inv_n = 1.f / ((float)a.HW * (float)a.cg.d);
+    group_sums<2>(a, p, sm, a.gamma, 1, sums, [&](float s) { return s * inv_n; });
     // dx = rstd (gamma g - mean(gamma g) - xhat mean(gamma g xhat)) = sc g + (x cd + c0)
     float cd[8], c0[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         const float rstd = grstd[gi[j]];
-        cd[j] = -rstd * rstd * sums[1][gi[j]] * inv_n;
-        c0[j] = fmaf(-mean[j], cd[j], -rstd * sums[0][gi[j]] * inv_n);
+        cd[j] = -rstd * rstd * sums[1][gi[j]];
+        c0[j] = fmaf(-mean[j], cd[j], -rstd * sums[0][gi[j]]);
     }
 #pragma unroll
     for (int i = 0; i < R; ++i) {
@@ -422,7 +424,7 @@ __global__ void __launch_bounds__(MAXT, WAVES) gn_bwd_tile(const GnArgs a) {
 }
 
 template <typename T, int ACT, bool RES>
-__global__ void __launch_bounds__(1024) gn_bwd_apply(const GnArgs a) {
+__global__ void __launch_bounds__(512) gn_bwd_apply(const GnArgs a) {
     extern __shared__ float sm[];            // [2][slab channels]
     __shared__ float sums[2][GN_MAX_GROUPS];
     const Place p = gn_place(a);
@@ -437,7 +439,7 @@ __global__ void __launch_bounds__(1024) gn_bwd_apply(const GnArgs a) {
         sm[t] = s;
     }
     __syncthreads();
-    group_sums<2>(a, p, sm, a.gamma, 1, sums);   // (a.ent is 1 in this launch)
+    group_sums<2>(a, p, sm, a.gamma, 1, sums, [](float s) { return s; });   // (a.ent is 1 in this launch)
     if (!p.live) return;
     int gi[8];
     chunk_groups(a, p, gi);
@@ -524,41 +526,45 @@ int check(const cvg_gn_desc* d, const char* who) {
     return 0;
 }
 
-// Registers hold rmax chunks per thread and tensor: 1024 threads have 128 registers each, 512 have 256.
+// One tile per (sample, slab) or several?  Registers hold rmax chunks per thread (512 threads of 16 bf16 chunks: 128 KB).
+//   Large batches: the widest slab, up to 128 bytes of a pixel row, that still fits and leaves 256 workgroups.  Measured
+//     forward on 256 x 32 x 32 x 128 bf16 with skip: 47 us at 64-byte slabs, 53 at 128 (too few workgroups), and on
+//     256 x 64 x 64 x 64 (512 KB a sample, so 32-byte slabs) 76 us against 87 for the two kernels of the tiled form.
+//   Few samples: a workgroup's own arithmetic counts, about 1.8 us per 1000 bf16 chunks (5 in f32), against some 5 us
+//     for a second launch: one 64 x 64 x 64 picture takes 11.4 us as 8 tiles of 4096 chunks and 9.2 as 64 of 512, the
+//     f32 crop 3 x 1961 x 72 13.9 forward and 17.7 backward as 27 tiles and 10.0 and 12.6 as 216.
 Plan plan(const cvg_gn_desc* d, bool backward, bool res) {
     Plan p;
     const int cg = d->C / d->G, unit = cg / gcd(cg, 8);             // chunks of 8 channels that hold whole groups
     const int all = d->C / 8;
     const bool bf = d->dtype == CVG_BF16;
     const int want = bf ? 8 : 4;                                    // 128 bytes of a pixel row
-    auto tmax = [](int nv) { return (nv & (nv - 1)) == 0 && nv <= 32 ? 1024 : 512; };   // (LDS rows where lanes do not fold)
-    auto rmax = [&](int threads) {
-        if (!backward) return (bf ? 8 : 4) * (threads <= 512 ? 2 : 1);
-        return (bf ? 16 : 8) / (res ? 2 : 1) / (threads <= 512 ? 1 : 4);
-    };
-    auto cap = [&](int nv) {                                        // rows one workgroup holds
-        int64_t best = 0;
-        for (int t = 512; t <= tmax(nv); t *= 2) { const int64_t c = (int64_t)(t / nv) * rmax(t); best = c > best ? c : best; }
-        return best;
-    };
-    int nv = unit;
-    while (nv < want && nv + unit <= all) nv += unit;
+    const int rmax = (bf ? 16 : 8) / (backward && res ? 2 : 1);
+    auto cap = [&](int nv) { return 512 / nv * rmax; };             // rows one workgroup holds
+    int wide = unit;
+    while (wide < want && wide + unit <= all) wide += unit;
+    int nv = wide;
     while (nv > unit && (d->HW > cap(nv) || (int64_t)d->B * ceil_div(all, nv) < 256)) nv -= unit;
-    const bool single = d->HW <= cap(nv);
-    if (!single) { nv = unit; while (nv < want && nv + unit <= all) nv += unit; }
+    const int64_t groups_of = (int64_t)d->B * ceil_div(all, nv);    // workgroups with one tile each
+    bool single = d->HW <= cap(nv);
+    if (groups_of < 256 && (int64_t)d->HW * nv > (bf ? 3072 : 1024)) single = false;
+    p.threads = nv <= 256 ? 256 : 512;
+    int rows = rmax;
+    if (single) {
+        while (p.threads < 512 && p.threads / nv * rmax < d->HW) p.threads *= 2;
+    } else {
+        const int64_t chunks = (int64_t)d->B * d->HW * all;
+        if (chunks > (1 << 19)) nv = wide;                          // more than 8 MB: bandwidth, not latency
+        p.threads = nv <= 256 ? 256 : 512;
+        // about 512 workgroups, and no more tiles per sample than one wave merges at once
+        rows = 1;
+        while (rows < rmax && (chunks > (int64_t)rows * 512 * 256 || (int64_t)rows * (p.threads / nv) * 64 < d->HW)) rows *= 2;
+        while (p.threads < 512 && chunks > (int64_t)rows * 1024 * 256) p.threads *= 2;
+    }
     p.nv = nv;
     p.nslab = ceil_div(all, nv);
-    p.threads = 256;
-    if (single) {
-        while (p.threads < tmax(nv) && (p.threads < nv || (int64_t)(p.threads / nv) * rmax(p.threads) < d->HW)) p.threads *= 2;
-    } else {
-        p.threads = nv <= 256 ? 256 : 512;
-        // enough tiles for every CU, otherwise as large as the registers allow
-        while (p.threads < tmax(nv) && (int64_t)d->B * p.nslab * ceil_div(d->HW, (p.threads / nv) * rmax(p.threads)) >= 1024) p.threads *= 2;
-    }
     p.rpp = p.threads / nv;
-    int need = ceil_div(d->HW, p.rpp);
-    if (need > rmax(p.threads)) need = rmax(p.threads);
+    const int need = min(rows, ceil_div(d->HW, p.rpp));
     p.R = 1;
     while (p.R < need) p.R *= 2;
     p.rows_tile = min(d->HW, p.R * p.rpp);
@@ -586,28 +592,27 @@ size_t ws_need(const cvg_gn_desc* d, const Plan& p, bool backward) {
     return p.tiles > 1 ? (size_t)d->B * d->G * p.tiles * 2 * 4 : 0;
 }
 
-// (the second number of a launch bound is waves per SIMD: 4 leave 128 registers)
+// (the second number of a launch bound is waves per SIMD: 4 leave 128 registers, 2 leave 256)
 template <typename T, int ACT>
 void run_fwd(const GnArgs& a, const Plan& p, hipStream_t s) {
     const int blocks = a.B * p.nslab * p.tiles;
     const size_t lds = (size_t)a.ent * p.nv * 8 * 4;
-    constexpr bool B = sizeof(T) == 2;
-    if (p.R == 1) gn_fwd_tile<T, ACT, 1, 1024, 4><<<blocks, p.threads, lds, s>>>(a);
-    else if (p.R <= 4) gn_fwd_tile<T, ACT, 4, 1024, 4><<<blocks, p.threads, lds, s>>>(a);
-    else if (p.R == 8) gn_fwd_tile<T, ACT, 8, B ? 1024 : 512, 4><<<blocks, p.threads, lds, s>>>(a);
-    else if constexpr (B) gn_fwd_tile<T, ACT, 16, 512, 4><<<blocks, p.threads, lds, s>>>(a);
+    constexpr int RMAX = sizeof(T) == 2 ? 16 : 8;
+    if (p.R == 1) gn_fwd_tile<T, ACT, 1, 512, 4><<<blocks, p.threads, lds, s>>>(a);
+    else if (p.R <= RMAX / 4) gn_fwd_tile<T, ACT, RMAX / 4, 512, 4><<<blocks, p.threads, lds, s>>>(a);
+    else if (p.R <= RMAX / 2) gn_fwd_tile<T, ACT, RMAX / 2, 512, 4><<<blocks, p.threads, lds, s>>>(a);
+    else gn_fwd_tile<T, ACT, RMAX, 512, 4><<<blocks, p.threads, lds, s>>>(a);
     if (p.tiles > 1) gn_fwd_apply<T, ACT><<<blocks, p.threads, 0, s>>>(a);
 }
 template <typename T, int ACT, bool RES>
 void run_bwd(GnArgs a, const Plan& p, hipStream_t s) {
     const int blocks = a.B * p.nslab * p.tiles;
     const size_t lds = (size_t)a.ent * p.nv * 8 * 4 * 2;
-    constexpr bool B = sizeof(T) == 2;
-    constexpr int R1024 = (B ? 4 : 2) / (RES ? 2 : 1), R512 = 4 * R1024;
-    if (p.R == 1) gn_bwd_tile<T, ACT, 1, RES, 1024, 4><<<blocks, p.threads, lds, s>>>(a);
-    else if (p.R <= R1024) gn_bwd_tile<T, ACT, R1024, RES, 1024, 4><<<blocks, p.threads, lds, s>>>(a);
-    else if (p.R <= 2 * R1024) gn_bwd_tile<T, ACT, 2 * R1024, RES, 512, 2><<<blocks, p.threads, lds, s>>>(a);
-    else gn_bwd_tile<T, ACT, R512, RES, 512, 2><<<blocks, p.threads, lds, s>>>(a);
+    constexpr int RMAX = (sizeof(T) == 2 ? 16 : 8) / (RES ? 2 : 1);
+    if (p.R == 1) gn_bwd_tile<T, ACT, 1, RES, 512, 4><<<blocks, p.threads, lds, s>>>(a);
+    else if (p.R <= RMAX / 4) gn_bwd_tile<T, ACT, RMAX / 4, RES, 512, 2><<<blocks, p.threads, lds, s>>>(a);
+    else if (p.R <= RMAX / 2) gn_bwd_tile<T, ACT, RMAX / 2, RES, 512, 2><<<blocks, p.threads, lds, s>>>(a);
+    else gn_bwd_tile<T, ACT, RMAX, RES, 512, 2><<<blocks, p.threads, lds, s>>>(a);
     if (p.tiles > 1) {
         a.ent = 1;
         gn_bwd_apply<T, ACT, RES><<<blocks, p.threads, (size_t)2 * p.nv * 8 * 4, s>>>(a);

@@ -4,11 +4,20 @@
 
 // ---- activations (CVG_ACT_*) --------------------------------------------------------------------------------
 // SiLU and the tanh form of GELU are both v * sigmoid(a(v)): a = v, and a = 2 sqrt(2/pi) (v + 0.044715 v^3) because
-// 0.5 (1 + tanh u) = sigmoid(2u).  EXACT (f32 tensors): expf and an IEEE division; otherwise v_exp_f32 / v_rcp_f32,
-// whose one-ulp-scale errors sit sixteen bits below the bf16 rounding that follows.
+// 0.5 (1 + tanh u) = sigmoid(2u).  The bf16 form takes v_exp_f32 and v_rcp_f32 as they are: their errors, and the
+// rounding of a log2(e), sit sixteen bits below the rounding that follows.  The f32 form (EXACT) adds the low part of
+// a log2(e) to first order and one Newton step of the reciprocal: 19 operations where expf and a division take 45, at an
+// error of about an ulp.  Beyond |a| = 87 the sigmoid is 0 or 1 to the last bit of f32.
 template <bool EXACT> __device__ __forceinline__ float fast_sigmoid(float a) {
-    if (EXACT) return 1.0f / (1.0f + expf(-a));
-    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(a * -1.4426950408889634f));
+    constexpr float L = -1.4426950408889634f, LLO = -1.9259629911266175e-8f;          // -log2(e) = L + LLO
+    if (!EXACT) return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(a * L));
+    const float x = __builtin_amdgcn_fmed3f(a, -87.f, 87.f);
+    const float t = x * L, lo = fmaf(x, LLO, fmaf(x, L, -t));
+    float e = __builtin_amdgcn_exp2f(t);
+    e = fmaf(e, lo * 0.6931471805599453f, e);
+    const float d = 1.0f + e, r = __builtin_amdgcn_rcpf(d);
+    const float p = fmaf(fmaf(-d, r, 1.0f), r, r);
+    return a < -87.f ? 0.f : p;
 }
 #define GELU_A 1.5957691216057308f       // 2 sqrt(2 / pi)
 #define GELU_B 0.044715f
@@ -59,6 +68,13 @@ template <bool EXACT> __device__ __forceinline__ void act_slope8(float (&v)[8], 
 }
 static inline bool act_known(int act) { return act >= CVG_ACT_NONE && act <= CVG_ACT_GELU; }
 
+// a barrier for LDS only: global loads and stores stay in flight across it
+__device__ __forceinline__ void lds_barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" : : : "memory");
+}
+
 __device__ __forceinline__ float wave_max(float v) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
@@ -97,3 +113,8 @@ __device__ __forceinline__ void raw_pack(Raw8<float>& r, const float (&v)[8]) {
 // keeps the unpacking of registers where it is written: hoisted above a branch, it would wait for every load at once
 __device__ __forceinline__ void pin(Raw8<bf16>& r) { asm volatile("" : "+v"(r.a)); }
 __device__ __forceinline__ void pin(Raw8<float>& r) { asm volatile("" : "+v"(r.a), "+v"(r.b)); }
+// keeps values in registers: where they come from LDS the compiler would rather read them again at every use
+__device__ __forceinline__ void pin(float (&v)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) asm volatile("" : "+v"(v[j]));
+}
