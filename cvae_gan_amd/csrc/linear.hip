@@ -5,6 +5,7 @@
 //   dx        A = dz (k contiguous), B = w read along its rows       M x K x N
 //   dw        A = dz, B = x, both read along their rows              N x K x M
 #include "rowops.h"
+#include <stdlib.h>
 
 namespace {
 
@@ -33,55 +34,61 @@ __device__ __forceinline__ void emit(const Epi& e, int m, int n, float v) {
 }
 
 // 8 consecutive columns of one row through the epilogue.  `whole`: all of them exist and every tensor takes 16-byte
-// accesses there.
+// accesses there.  Bias and residual are loaded by the caller (zeros where there are none), well before they are needed.
+__device__ __forceinline__ void load_bias8(const Epi& e, int n, int n_end, bool whole, float (&b)[8]) {
+    if (e.bias && whole) {
+        load8<float>(e.bias + n, b);
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) b[j] = e.bias && n + j < n_end ? e.bias[n + j] : 0.f;
+}
 template <typename T>
-__device__ __forceinline__ void emit8(const Epi& e, int m, int n, int n_end, bool whole, float (&v)[8]) {
+__device__ __forceinline__ void load_res8(const Epi& e, int m, int n, int n_end, bool whole, float (&q)[8]) {
+    const T* r = (const T*)e.res + (size_t)m * e.res_ld + n;
+    if (whole) {
+        load8<T>(r, q);
+    } else if (n + 8 <= n_end) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) q[j] = to_f32(r[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) q[j] = n + j < n_end ? to_f32(r[j]) : 0.f;
+    }
+}
+template <typename T>
+__device__ __forceinline__ void emit8(const Epi& e, int m, int n, int n_end, bool whole, float (&v)[8], const float (&b)[8], const float (&q)[8]) {
     constexpr bool EXACT = sizeof(T) == 4;
-    if (!whole) {
-        float b[8], q[8];                // (all loads before the first use)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            b[j] = e.bias && n + j < n_end ? e.bias[n + j] : 0.f;
-            q[j] = e.res && n + j < n_end ? to_f32(((const T*)e.res)[(size_t)m * e.res_ld + n + j]) : 0.f;
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] += b[j];
-        if (e.pre)
+    for (int j = 0; j < 8; ++j) v[j] += b[j];
+    if (e.pre) {
+        if (whole) {
+            if (e.pre_f32) store8<float>((float*)e.pre + (size_t)m * e.pre_ld + n, v);
+            else store8<T>((T*)e.pre + (size_t)m * e.pre_ld + n, v);
+        } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
                 if (n + j < n_end) {
                     if (e.pre_f32) ((float*)e.pre)[(size_t)m * e.pre_ld + n + j] = v[j];
                     else ((T*)e.pre)[(size_t)m * e.pre_ld + n + j] = from_f32<T>(v[j]);
                 }
-        act_value8<EXACT>(v, e.act);
+        }
+    }
+    act_value8<EXACT>(v, e.act);
+    if (e.res)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] += q[j];
+    if (whole) {
+        if (e.out_f32) store8<float>((float*)e.out + (size_t)m * e.out_ld + n, v);
+        else store8<T>((T*)e.out + (size_t)m * e.out_ld + n, v);
+    } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
             if (n + j < n_end) {
-                const float o = v[j] + q[j];
-                if (e.out_f32) ((float*)e.out)[(size_t)m * e.out_ld + n + j] = o;
-                else ((T*)e.out)[(size_t)m * e.out_ld + n + j] = from_f32<T>(o);
+                if (e.out_f32) ((float*)e.out)[(size_t)m * e.out_ld + n + j] = v[j];
+                else ((T*)e.out)[(size_t)m * e.out_ld + n + j] = from_f32<T>(v[j]);
             }
-        return;
     }
-    if (e.bias) {
-        float b[8];
-        load8<float>(e.bias + n, b);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] += b[j];
-    }
-    if (e.pre) {
-        if (e.pre_f32) store8<float>((float*)e.pre + (size_t)m * e.pre_ld + n, v);
-        else store8<T>((T*)e.pre + (size_t)m * e.pre_ld + n, v);
-    }
-    act_value8<EXACT>(v, e.act);
-    if (e.res) {
-        float q[8];
-        load8<T>((const T*)e.res + (size_t)m * e.res_ld + n, q);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] += q[j];
-    }
-    if (e.out_f32) store8<float>((float*)e.out + (size_t)m * e.out_ld + n, v);
-    else store8<T>((T*)e.out + (size_t)m * e.out_ld + n, v);
 }
 
 // D[m][n] = sum_k A(m, k) B(n, k) for one output tile, or one K range of it.
@@ -194,10 +201,15 @@ struct Operand {
 // Tile kernel: BM x BN per workgroup of WR x WC waves.  Two LDS stages of 128 bytes of k, filled by direct-to-LDS loads
 // two stages ahead; fragments are read one 16-k step ahead of the MFMAs that use them, across the stage border too, so
 // the one barrier of a stage sits between the last fragment reads of a stage and the MFMAs on them.
+// LDS stages in flight: two of 64 KB for the large tile; the small tile, whose stages are over in a fraction of a load's
+// latency, runs four
+template <int BM> constexpr int ring() { return BM == 64 ? 4 : 2; }
 template <typename T, int BM, int BN, int WR, int WC> struct TileLds {
-    static constexpr int STAGES = 2 * (BM + BN) * 128, EPI = WR * WC * 32 * (BN / WC * 4 + 16);
+    static constexpr int STAGES = ring<BM>() * (BM + BN) * 128, EPI = WR * WC * 32 * (BN / WC * 4 + 16);
     static constexpr int BYTES = STAGES > EPI ? STAGES : EPI;
 };
+struct Yes { static constexpr bool value = true; };
+struct No { static constexpr bool value = false; };
 template <typename T, int BM, int BN, int WR, int WC, bool ACOL, bool BCOL>
 __device__ __forceinline__ void tile_body(const GemmArgs& a, int id, int slice, char* lds) {
     constexpr int NW = WR * WC, WM = BM / WR, WN = BN / WC, TI = WM / 32, TJ = WN / 32;
@@ -205,7 +217,7 @@ __device__ __forceinline__ void tile_body(const GemmArgs& a, int id, int slice, 
     typedef Operand<T, BN, NW, BCOL> OB;
     typedef typename Elem<T>::frag frag;
     constexpr int BK = OA::BK, NS = BK / 16;
-    constexpr int STAGE = OA::BYTES + OB::BYTES;
+    constexpr int STAGE = OA::BYTES + OB::BYTES, D = ring<BM>();
     constexpr int EP = WN * 4 + 16;                                // epilogue: 32 rows of the wave's columns, f32
     // workgroups go round-robin over the 8 dies, each with its own L2: give every die a run of neighbouring tiles, walked
     // in strips of 4 tile rows
@@ -220,6 +232,13 @@ __device__ __forceinline__ void tile_body(const GemmArgs& a, int id, int slice, 
     const int k0 = slice * a.k_split, k_len = min(a.K - k0, a.k_split);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int wm = (wave / WC) * WM, wn = (wave % WC) * WN;
+
+    // this lane's columns in the epilogue; their bias is on its way while the products are taken
+    constexpr int LPR = WN / 8, RPP = 64 / LPR, PASSES = 32 / RPP;      // lanes per row, rows per pass
+    const int cl = (lane % LPR) * 8, rl = lane / LPR, n = n0 + wn + cl;
+    const bool whole = a.vec && n + 8 <= a.N;
+    float bias[8];
+    load_bias8(a.e, n, a.N, whole, bias);
 
     OA oa;
     OB ob;
@@ -243,8 +262,8 @@ __device__ __forceinline__ void tile_body(const GemmArgs& a, int id, int slice, 
             for (int j = 0; j < TJ; ++j) far[i][j] = acc[i][j];
     }
     const int stages = (k_len + BK - 1) / BK, full = k_len / BK;
-    auto issue = [&](int st) {
-        char* base = lds + (st & 1) * STAGE;
+    auto issue = [&](int st, int buf) {
+        char* base = lds + buf * STAGE;
         if (st < full) {
             oa.template issue<true>(base, 0);
             ob.template issue<true>(base + OA::BYTES, 0);
@@ -254,14 +273,30 @@ __device__ __forceinline__ void tile_body(const GemmArgs& a, int id, int slice, 
         }
     };
     frag fa[2][TI], fb[2][TJ];
-    auto read = [&](int st, int s, int into) {
-        const char* base = lds + (st & 1) * STAGE;
+    auto read = [&](int buf, int s, int into) {
+        const char* base = lds + buf * STAGE;
 #pragma unroll
         for (int i = 0; i < TI; ++i) fa[into][i] = OA::frag(base, wm + i * 32, s, lane);
 #pragma unroll
         for (int j = 0; j < TJ; ++j) fb[into][j] = OB::frag(base + OA::BYTES, wn + j * 32, s, lane);
     };
+    constexpr bool MIX = TI * TJ >= 16;
     auto multiply = [&](int from) {
+        if constexpr (MIX) {
+#pragma unroll
+            for (int i = 0; i < TI; ++i)
+#pragma unroll
+                for (int j = 0; j < TJ; ++j) mma32(acc[i][j], fa[from][i], fb[from][j]);
+#pragma unroll
+            for (int g = 0; g < 8; ++g) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x020, 2, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            return;
+        }
         __builtin_amdgcn_sched_barrier(0);
         __builtin_amdgcn_s_setprio(1);
 #pragma unroll
@@ -283,55 +318,56 @@ __device__ __forceinline__ void tile_body(const GemmArgs& a, int id, int slice, 
             }
         }
     };
-    // the border between stage st and st + 1: this wave's reads of st have arrived and so has its part of st + 1; behind
-    // the barrier that holds for every wave, so st + 1 may be read and st overwritten
-    auto border = [&]() {
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" : : : "memory");
+    // The border between stage st and st + 1: this wave's reads of st have arrived and so has its part of st + 1; behind
+    // the barrier that holds for every wave, so st + 1 may be read and st overwritten.  While only whole stages are in
+    // flight the D - 2 stages behind st + 1 stay so; a partial one takes an unknown number of loads.
+    constexpr int L = OA::NL + OB::NL;
+    auto border = [&](auto steady) {
+        if constexpr (decltype(steady)::value) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"((D - 2) * L) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" : : : "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" : : : "memory");
     };
-    constexpr int L = OA::NL + OB::NL;
-    issue(0);
-    if (stages > 1) {
-        issue(1);
-        if (stages - 1 < full || stages > 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"(L) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" : : : "memory");       // (a partial stage may take fewer loads)
-    } else {
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" : : : "memory");
-    }
+    for (int st = 0; st < D && st < stages; ++st) issue(st, st);
+    if (full >= D) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"((D - 1) * L) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" : : : "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" : : : "memory");
     read(0, 0, 0);
-    int st = 0;
-    for (; st + 2 < full; ++st) {
+    int st = 0, buf = 0;
+    for (; st + D < full; ++st) {
+        const int after = buf + 1 == D ? 0 : buf + 1;
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
             if (s < NS - 1) {
-                read(st, s + 1, (s + 1) & 1);
+                read(buf, s + 1, (s + 1) & 1);
             } else {
-                border();
-                read(st + 1, 0, (s + 1) & 1);
-                char* base = lds + (st & 1) * STAGE;
+                border(Yes{});
+                read(after, 0, (s + 1) & 1);
+                char* base = lds + buf * STAGE;
                 oa.template issue<true>(base, 0);
                 ob.template issue<true>(base + OA::BYTES, 0);
             }
             multiply(s & 1);
         }
         fold(st);
+        buf = after;
     }
     for (; st < stages; ++st) {
+        const int after = buf + 1 == D ? 0 : buf + 1;
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
             if (s < NS - 1) {
-                read(st, s + 1, (s + 1) & 1);
+                read(buf, s + 1, (s + 1) & 1);
             } else if (st + 1 < stages) {
-                border();
-                read(st + 1, 0, (s + 1) & 1);
-                if (st + 2 < stages) issue(st + 2);
+                border(No{});
+                read(after, 0, (s + 1) & 1);
+                if (st + D < stages) issue(st + D, buf);
             }
             multiply(s & 1);
         }
         fold(st);
+        buf = after;
     }
     if constexpr (FOLD) {
 #pragma unroll
@@ -344,10 +380,9 @@ __device__ __forceinline__ void tile_body(const GemmArgs& a, int id, int slice, 
     // epilogue: 32 x WN blocks through LDS, so that a lane ends up with 8 consecutive columns
     __syncthreads();
     char* ep = lds + wave * 32 * EP;
-    constexpr int LPR = WN / 8, RPP = 64 / LPR;                    // lanes per row, rows per pass
-    const int l31 = lane & 31, h = lane >> 5, cl = (lane % LPR) * 8, rl = lane / LPR;
-    const int n = n0 + wn + cl;
-    const bool whole = a.vec && n + 8 <= a.N;
+    const int l31 = lane & 31, h = lane >> 5;
+    const bool has_res = !a.slab && a.e.res;
+    constexpr int PG = PASSES < 4 ? PASSES : 4;                    // passes whose residual is loaded together
 #pragma unroll
     for (int i = 0; i < TI; ++i) {
 #pragma unroll
@@ -357,19 +392,28 @@ __device__ __forceinline__ void tile_body(const GemmArgs& a, int id, int slice, 
                 *(float*)(ep + ((e & 3) + 8 * (e >> 2) + 4 * h) * EP + (j * 32 + l31) * 4) = acc[i][j][e];
         // (the region is this wave's own: its LDS accesses complete in order)
 #pragma unroll 1
-        for (int r = 0; r < 32; r += RPP) {
-            const int m = m0 + wm + i * 32 + r + rl;
-            float v[8];
-            load8<float>((const float*)(ep + (r + rl) * EP + cl * 4), v);
-            if (m >= a.M || n >= a.N) continue;
-            if (a.slab) {
-                float* o = a.slab + ((size_t)slice * a.M + m) * a.N + n;
-                if (n + 8 <= a.N && (a.N & 3) == 0) store8<float>(o, v);
-                else
-                    for (int j = 0; j < 8; ++j)
-                        if (n + j < a.N) o[j] = v[j];
-            } else {
-                emit8<T>(a.e, m, n, a.N, whole, v);
+        for (int r0 = 0; r0 < PASSES; r0 += PG) {
+            const int mb = m0 + wm + i * 32 + r0 * RPP + rl;
+            float q[PG][8];
+            if (has_res && n < a.N) {
+#pragma unroll
+                for (int r = 0; r < PG; ++r) load_res8<T>(a.e, min(mb + r * RPP, a.M - 1), n, a.N, whole, q[r]);
+            }
+#pragma unroll
+            for (int r = 0; r < PG; ++r) {
+                const int m = mb + r * RPP;
+                float v[8];
+                load8<float>((const float*)(ep + ((r0 + r) * RPP + rl) * EP + cl * 4), v);
+                if (m >= a.M || n >= a.N) continue;
+                if (a.slab) {
+                    float* o = a.slab + ((size_t)slice * a.M + m) * a.N + n;
+                    if (n + 8 <= a.N && (a.N & 3) == 0) store8<float>(o, v);
+                    else
+                        for (int j = 0; j < 8; ++j)
+                            if (n + j < a.N) o[j] = v[j];
+                } else {
+                    emit8<T>(a.e, m, n, a.N, whole, v, bias, q[r]);
+                }
             }
         }
     }
@@ -379,6 +423,83 @@ template <typename T, int BM, int BN, int WR, int WC, bool ACOL, bool BCOL>
 __global__ void __launch_bounds__(WR * WC * 64) gemm_tile(const GemmArgs a) {
     __shared__ __attribute__((aligned(1024))) char lds[TileLds<T, BM, BN, WR, WC>::BYTES];
     tile_body<T, BM, BN, WR, WC, ACOL, BCOL>(a, blockIdx.x, blockIdx.y, lds);
+}
+
+// ---- few rows: M <= 16 MT ------------------------------------------------------------------------------------
+// The weights are all there is to read.  A workgroup takes 16 of their rows; its eight waves take turns along k, 64 values
+// (a whole cache line of a bf16 row) at a time, straight from memory into 16 x 16 MFMA fragments: lane (r, q) holds k
+// values 16 q .. 16 q + 15 of the unit, of weight row r and of x row r alike, so any order of k inside the unit is right as
+// long as both operands share it.  x rows beyond M are zero.  The waves' sums meet in LDS in wave order; no second launch.
+// One token through 4096 x 4096 bf16: 34 MB.
+template <typename T> struct Unit;                                // 16 consecutive k of one row
+template <> struct Unit<bf16> { u32x4 a[2]; };
+template <> struct Unit<float> { u32x4 a[4]; };
+template <typename T, bool ALIGNED>
+__device__ __forceinline__ void unit_load(Unit<T>& u, const T* row, int k, int K, bool live) {
+    constexpr int PER = 16 / sizeof(T), NV = 16 / PER;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int kk = k + i * PER;
+        u.a[i] = u32x4{0, 0, 0, 0};
+        if constexpr (ALIGNED) {
+            if (live && kk < K) u.a[i] = *(const u32x4*)(row + kk);       // (K is a multiple of 16 bytes)
+        } else if (live) {
+            T t[PER];
+#pragma unroll
+            for (int j = 0; j < PER; ++j) t[j] = kk + j < K ? row[kk + j] : from_f32<T>(0.f);
+            u.a[i] = __builtin_bit_cast(u32x4, *(T (*)[PER])t);
+        }
+    }
+}
+__device__ __forceinline__ void unit_mma(f32x4& acc, const Unit<bf16>& w, const Unit<bf16>& x) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w.a[i]), __builtin_bit_cast(bf16x8, x.a[i]), acc, 0, 0, 0);
+}
+__device__ __forceinline__ void unit_mma(f32x4& acc, const Unit<float>& w, const Unit<float>& x) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(w.a[i][j]), __uint_as_float(x.a[i][j]), acc, 0, 0, 0);
+}
+template <typename T, int MT, bool ALIGNED>
+__global__ void __launch_bounds__(512) few_rows(const GemmArgs a) {
+    constexpr int U = (sizeof(T) == 2 && ALIGNED ? 8 : 4) / MT;   // units in flight per wave
+    __shared__ float red[8][MT][16][17];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4, n0 = blockIdx.x * 16;
+    const T* w = (const T*)a.B + (size_t)min(n0 + r, a.N - 1) * a.ldb;
+    f32x4 acc[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int k0 = wave * 64; k0 < a.K; k0 += U * 512) {
+        Unit<T> uw[U], ux[U][MT];
+#pragma unroll
+        for (int u = 0; u < U; ++u) unit_load<T, ALIGNED>(uw[u], w, k0 + u * 512 + q * 16, a.K, true);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+                unit_load<T, ALIGNED>(ux[u][t], (const T*)a.A + (size_t)min(t * 16 + r, a.M - 1) * a.lda, k0 + u * 512 + q * 16, a.K, t * 16 + r < a.M);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) unit_mma(acc[t], uw[u], ux[u][t]);
+    }
+    // lane (r, q): x row r, weight rows 4 q .. 4 q + 3
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) red[wave][t][r][4 * q + i] = acc[t][i];
+    __syncthreads();
+    for (int i = threadIdx.x; i < MT * 256; i += 512) {
+        const int n = i & 15, m = i >> 4;
+        if (m >= a.M || n0 + n >= a.N) continue;
+        float v = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v += red[j][m >> 4][m & 15][n];
+        emit<T>(a.e, m, n0 + n, v);
+    }
 }
 
 // column sums of [P][N] partial rows: 32 columns by `blockDim / 32` row lanes
@@ -457,7 +578,12 @@ __device__ __forceinline__ void slab_sum_body(const GemmArgs& a, int splits, int
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] += sm[q * per_blk + lo][j];
     }
-    if (live) emit8<T>(a.e, m, n, a.N, a.vec && n + 8 <= a.N, v);
+    if (!live) return;
+    const bool whole = a.vec && n + 8 <= a.N;
+    float b[8], q8[8];
+    load_bias8(a.e, n, a.N, whole, b);
+    if (a.e.res) load_res8<T>(a.e, m, n, a.N, whole, q8);
+    emit8<T>(a.e, m, n, a.N, whole, v, b, q8);
 }
 struct SlabJob { GemmArgs a; int splits, zl, blocks; };
 template <typename T>
@@ -478,8 +604,13 @@ __device__ __forceinline__ void pad_body(const void* in, size_t ld, void* out, i
     const int r = (int)(i / n8), c = (int)(i % n8) * 8;
     const T* q = (const T*)in + (size_t)r * ld + c;
     float v[8];
+    if (c + 8 <= width) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = c + j < width ? to_f32(q[j]) : 0.f;
+        for (int j = 0; j < 8; ++j) v[j] = to_f32(q[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = c + j < width ? to_f32(q[j]) : 0.f;
+    }
     store8<T>((T*)out + (size_t)r * out_ld + c, v);
 }
 struct PadJob { const void* in; void* out; size_t ld; int rows, width, out_ld, blocks; };
@@ -515,6 +646,12 @@ __device__ __forceinline__ void dz_body(const DzJob& a, int blk, float (*sm)[264
                 if (whole) {
                     load8<T>(gp, g[u]);
                     if (a.act != CVG_ACT_NONE) load8<P>(qp, q[u]);
+                } else if (c + 8 <= a.N) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        g[u][j] = to_f32(gp[j]);
+                        if (a.act != CVG_ACT_NONE) q[u][j] = to_f32(qp[j]);
+                    }
                 } else {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
@@ -575,6 +712,7 @@ size_t round_up(size_t v, size_t to) { return (v + to - 1) / to * to; }
 size_t max_sz(size_t a, size_t b) { return a > b ? a : b; }
 
 // the tile kernel's lane offsets span 256 rows in 31 bits
+constexpr int FEW_ROWS = 32;
 constexpr int MAX_WIDTH = 2000000;
 constexpr size_t MAX_PITCH = ((size_t)1 << 31) / 256 - 64;       // bytes
 
@@ -600,8 +738,8 @@ int check(const cvg_linear_desc* d, const char* who) {
 // cycle chip-wide) and a launch.
 struct Tile { int cfg, splits, k_split; double t; };
 struct TileShape { int bm, bn, occ; double mfma; };
-const TileShape TILES[2][3] = {{{0, 0, 0, 0}, {128, 128, 2, 4096 / .85}, {64, 64, 3, 1024 / .7}},
-                               {{256, 256, 1, 2048 / .8}, {128, 128, 2, 512 / .6}, {64, 64, 4, 128 / .4}}};
+const TileShape TILES[2][3] = {{{0, 0, 0, 0}, {128, 128, 2, 4096 / .85}, {64, 64, 2, 1024 / .7}},
+                               {{256, 256, 1, 2048 / .8}, {128, 128, 2, 512 / .6}, {64, 64, 2, 128 / .4}}};
 Tile choose_split(int dtype, int c, int64_t M, int64_t N, int64_t K) {
     const TileShape& sh = TILES[dtype == CVG_BF16][c];
     const int bk = dtype == CVG_BF16 ? 64 : 32;
@@ -710,7 +848,10 @@ int sum_slabs(const SlabJob& one, const SlabJob& two, hipStream_t s) {
 template <typename T>
 int multiply(GemmArgs& a, bool acol, bool bcol, const Tile& t, hipStream_t s) {
     if (t.cfg == 0) {
-        if constexpr (sizeof(T) == 2) launch_tile<T, 256, 256, 2, 4>(a, acol, bcol, t.splits, s);
+        if constexpr (sizeof(T) == 2) {
+            if (getenv("LIN_4W")) launch_tile<T, 256, 256, 2, 2>(a, acol, bcol, t.splits, s);
+            else launch_tile<T, 256, 256, 2, 4>(a, acol, bcol, t.splits, s);
+        }
     } else if (t.cfg == 1) {
         launch_tile<T, 128, 128, 2, 2>(a, acol, bcol, t.splits, s);
     } else {
@@ -723,17 +864,17 @@ int multiply(GemmArgs& a, bool acol, bool bcol, const Tile& t, hipStream_t s) {
 // Workspaces: dz, partial column sums, padded copies, slabs.  The sizes do not depend on pitches or alignment, so one
 // workspace serves every call of the same shape.
 size_t fwd_ws(const cvg_linear_desc* d) {
-    if (d->M == 0) return 0;
+    if (d->M <= FEW_ROWS) return 0;
     const size_t es = es_of(d->dtype);
     return padded_bytes(d->M, d->K, es) + padded_bytes(d->N, d->K, es) + slab_of(choose(d->dtype, d->M, d->N, d->K), d->M, d->N);
 }
 int dz_rows_blk(const cvg_linear_desc* d) {
-    // about 2048 workgroups where there are rows enough, at least 32 rows each
+    // about 2048 workgroups where there are rows enough, at most 128 rows of partial sums, at least 8 rows each
     const int64_t cols = ceil_div(d->N, 256);
     int64_t blks = 2048 / cols > 0 ? 2048 / cols : 1;
     if (blks > 128) blks = 128;
     const int64_t rb = ceil_div(d->M, blks);
-    return (int)(rb < 32 ? 32 : round_up(rb, 32));
+    return (int)(rb < 32 ? round_up(rb, 8) : round_up(rb, 32));
 }
 size_t part_bytes(const cvg_linear_desc* d) { return round_up((size_t)ceil_div(d->M, dz_rows_blk(d)) * d->N * 4, 256); }
 size_t bwd_ws(const cvg_linear_desc* d) {
@@ -748,15 +889,28 @@ template <typename T>
 int forward(const cvg_linear_desc* d, const void* x, const void* w, const float* bias, const void* res, void* y, void* pre, char* ws,
             hipStream_t s) {
     Rows X{x, ld_of(d->x_ld, d->K), d->M, d->K}, W{w, ld_of(d->w_ld, d->K), d->N, d->K};
+    Epi e{};
+    e.bias = bias; e.res = res; e.pre = pre; e.out = y; e.act = d->act;
+    e.out_f32 = 0; e.pre_f32 = sizeof(T) == 2 && d->pre_dtype == CVG_F32;
+    e.res_ld = ld_of(d->res_ld, d->N); e.pre_ld = ld_of(d->pre_ld, d->N); e.out_ld = ld_of(d->y_ld, d->N);
+    if (d->M <= FEW_ROWS) {
+        GemmArgs a{};
+        a.A = X.p; a.B = W.p; a.lda = X.ld; a.ldb = W.ld; a.M = d->M; a.N = d->N; a.K = d->K; a.e = e;
+        const bool al = fits(X, sizeof(T)) && fits(W, sizeof(T));
+        const int blocks = ceil_div(d->N, 16);
+        if (d->M <= 16) {
+            if (al) few_rows<T, 1, true><<<blocks, 512, 0, s>>>(a); else few_rows<T, 1, false><<<blocks, 512, 0, s>>>(a);
+        } else {
+            if (al) few_rows<T, 2, true><<<blocks, 512, 0, s>>>(a); else few_rows<T, 2, false><<<blocks, 512, 0, s>>>(a);
+        }
+        CVG_LAUNCH_CHECK();
+        return 0;
+    }
     const PadJob p0 = pad_job<T>(X, ws), p1 = pad_job<T>(W, ws);
     if (p0.blocks + p1.blocks) {
         prepare<T, T><<<p0.blocks + p1.blocks, 256, 0, s>>>(DzJob{}, p0, p1);
         CVG_LAUNCH_CHECK();
     }
-    Epi e{};
-    e.bias = bias; e.res = res; e.pre = pre; e.out = y; e.act = d->act;
-    e.out_f32 = 0; e.pre_f32 = sizeof(T) == 2 && d->pre_dtype == CVG_F32;
-    e.res_ld = ld_of(d->res_ld, d->N); e.pre_ld = ld_of(d->pre_ld, d->N); e.out_ld = ld_of(d->y_ld, d->N);
     const Tile t = choose(Elem<T>::DT, d->M, d->N, d->K);
     GemmArgs a = gemm_args<T>(X, false, W, false, d->M, d->N, d->K, e, t, ws);
     return multiply<T>(a, false, false, t, s);
@@ -846,7 +1000,7 @@ int cvg_linear_act_fwd(const cvg_linear_desc* d, const void* x, const void* w, c
     for (const void* p : ps) CVG_CHECK((uintptr_t)p % es == 0, "linear_act_fwd: misaligned tensor");
     CVG_CHECK((uintptr_t)pre % es_of(d->pre_dtype) == 0 && (uintptr_t)bias % 4 == 0, "linear_act_fwd: misaligned tensor");
     const size_t need = fwd_ws(d);
-    CVG_CHECK(ws && ws_bytes >= need && aligned16(ws), "linear_act_fwd: workspace of %zu bytes, need %zu", ws_bytes, need);
+    CVG_CHECK(need == 0 || (ws && ws_bytes >= need && aligned16(ws)), "linear_act_fwd: workspace of %zu bytes, need %zu", ws_bytes, need);
     hipStream_t st = (hipStream_t)s;
     return d->dtype == CVG_BF16 ? forward<bf16>(d, x, w, bias, res, y, pre, (char*)ws, st)
                                 : forward<float>(d, x, w, bias, res, y, pre, (char*)ws, st);
