@@ -5,7 +5,6 @@
 //   dx        A = dz (k contiguous), B = w read along its rows       M x K x N
 //   dw        A = dz, B = x, both read along their rows              N x K x M
 #include "rowops.h"
-#include <stdlib.h>
 
 namespace {
 
@@ -98,6 +97,7 @@ struct GemmArgs {
     int M, N, K;
     int ra, rb;                      // rows of A and B that may be addressed (the padded count where k is strided)
     int tiles_m, tiles_n, k_split;   // k_split: K range of one grid.y slice (a multiple of the K step)
+    int fast;                        // `vec`, whole 8-column groups only, and pitches that Streams takes
     int vec;                         // every tensor of the epilogue takes 16-byte accesses at multiples of 8 columns
     float* slab;                     // [splits][M][N] partial sums instead of the epilogue, or null
     Epi e;
@@ -106,11 +106,14 @@ struct GemmArgs {
 typedef __attribute__((address_space(3))) void* lds_dst;
 
 // One operand of the tile kernel: ROWS rows of the output dimension, BK = 128 bytes of k per stage.
-//   k contiguous (COL = false): LDS holds [ROWS][128 bytes]; the 16-byte chunk c of row r lies at c ^ (r & 7), so the 8 rows
-//     that one pass of a 16-byte LDS read touches lie in 8 different chunk columns, i.e. in all banks.
+//   k contiguous (COL = false): LDS holds [ROWS][128 bytes]; the 16-byte chunk c of row r lies at c ^ (r >> 1 & 7).  A
+//     16-byte LDS read is served 16 lanes at a time ({0-3, 12-15, 20-27}, {4-11, 16-19, 28-31} and the same of the upper
+//     half) over 64 banks of 4 bytes: the 16 rows of a group are 8 even and 8 odd ones, two rows fill the banks once, and
+//     r >> 1 takes all 8 values in each half.  (c ^ (r & 7) collides two by two: 45 % of the LDS cycles of a 256 x 256 tile.)
 //   k strided (COL = true): LDS holds [BK][ROWS]; bf16 fragments come out of ds_read_b64_tr_b16 (TrLoad), whose lanes read
 //     8 k-rows of 64 bytes at once; 64-byte block b of k-row k lies at b ^ (k & 3 | (k >> 3 & 1) << 2) (as many bits as there
-//     are blocks), which spreads those rows over the banks.  f32 reads single dwords, consecutive along the row.
+//     are blocks), which spreads those rows over the banks.  f32 reads single dwords, 32 columns of k-rows k and k + 8 at
+//     once: the upper one's 128-byte blocks are exchanged in pairs.
 // The swizzle is applied to the address a lane LOADS FROM: the direct-to-LDS load writes lane l at base + 16 l.
 template <typename T, int ROWS, int NWAVES, bool COL>
 struct Operand {
@@ -129,7 +132,7 @@ struct Operand {
     // first k, inside the stage, of load i of this lane
     __device__ __forceinline__ int k_of(int i) const {
         const int o = (i * NWAVES + wave) * 1024 + (tid & 63) * 16;
-        if constexpr (!COL) return (((o >> 4) & 7) ^ ((o >> 7) & 7)) * (16 / ES);
+        if constexpr (!COL) return (((o >> 4) ^ (o >> 8)) & 7) * (16 / ES);
         else return o / RB;
     }
     __device__ __forceinline__ void init(const void* p, size_t ld, int row0, int rows, int k0, int tid_) {
@@ -145,38 +148,49 @@ struct Operand {
                 off[i] = (int)((size_t)r * ld * ES) + k_of(i) * ES;
             } else {
                 const int k = o / RB, c = (o % RB) >> 4;
-                const int cs = ES == 2 ? (((c >> 2) ^ swz(k)) << 2) | (c & 3) : c;
+                const int cs = ES == 2 ? (((c >> 2) ^ swz(k)) << 2) | (c & 3) : c ^ (k & 8);
                 int g = cs * (16 / ES);
                 if (row0 + g >= rows) g = 0;                      // (rows is a multiple of the chunk)
                 off[i] = (int)((size_t)k * ld * ES) + g * ES;
             }
         }
     }
-    // FULL: the whole stage lies inside the k range; otherwise it is zero from k_left on
-    template <bool FULL> __device__ __forceinline__ void issue(char* lds, int k_left) {
+    // load i of a stage.  FULL: the whole stage lies inside the k range; otherwise it is zero from k_left on
+    template <bool FULL> __device__ __forceinline__ void load(char* lds, int i, int k_left) {
 #ifdef __HIP_DEVICE_COMPILE__
         const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, 0x7fffffff, 0x00020000);
-#pragma unroll
-        for (int i = 0; i < NL; ++i) {
-            char* to = lds + (i * NWAVES + wave) * 1024;
-            if (FULL || k_of(i) < k_left)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_dst)to, 16, off[i], 0, 0, 0);
-            else
-                *(u32x4*)(to + (tid & 63) * 16) = u32x4{0, 0, 0, 0};
-        }
+        char* to = lds + (i * NWAVES + wave) * 1024;
+        if (FULL || k_of(i) < k_left)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_dst)to, 16, off[i], 0, 0, 0);
+        else
+            *(u32x4*)(to + (tid & 63) * 16) = u32x4{0, 0, 0, 0};
 #endif
-        base += step;
+        if (i == NL - 1) base += step;
+    }
+    // the same by way of registers: fetch has the load under way, put writes it to LDS
+    template <bool FULL> __device__ __forceinline__ u32x4 fetch(int i, int k_left) {
+        u32x4 v = {0, 0, 0, 0};
+#ifdef __HIP_DEVICE_COMPILE__
+        const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, 0x7fffffff, 0x00020000);
+        if (FULL || k_of(i) < k_left) v = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, off[i], 0, 0));
+#endif
+        if (i == NL - 1) base += step;
+        return v;
+    }
+    __device__ __forceinline__ void put(char* lds, int i, u32x4 v) const {
+        *(u32x4*)(lds + (i * NWAVES + wave) * 1024 + (tid & 63) * 16) = v;
     }
     // fragment of rows r0 .. r0 + 31, k-step s (16 values: slot (h, j) = k 8 h + j)
     __device__ __forceinline__ static typename Elem<T>::frag frag(const char* lds, int r0, int s, int lane) {
         const int l31 = lane & 31, h = lane >> 5;
         if constexpr (!COL) {
             const char* q = lds + (r0 + l31) * 128;
+            const int f = (l31 >> 1) & 7;
             if constexpr (ES == 2) {
-                return *(const bf16x8*)(q + (((2 * s + h) ^ (l31 & 7)) << 4));
+                return *(const bf16x8*)(q + (((2 * s + h) ^ f) << 4));
             } else {
-                const f32x4 a = *(const f32x4*)(q + (((4 * s + 2 * h) ^ (l31 & 7)) << 4));
-                const f32x4 b = *(const f32x4*)(q + (((4 * s + 2 * h + 1) ^ (l31 & 7)) << 4));
+                const f32x4 a = *(const f32x4*)(q + (((4 * s + 2 * h) ^ f) << 4));
+                const f32x4 b = *(const f32x4*)(q + (((4 * s + 2 * h + 1) ^ f) << 4));
                 return f32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
             }
         } else {
@@ -191,18 +205,96 @@ struct Operand {
             } else {
                 f32x8 r;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) r[j] = *(const float*)(lds + (16 * s + 8 * h + j) * RB + (r0 + l31) * 4);
+                for (int j = 0; j < 8; ++j) r[j] = *(const float*)(lds + (16 * s + 8 * h + j) * RB + ((r0 + l31) ^ (h << 5)) * 4);
                 return r;
             }
         }
     }
 };
 
-// Tile kernel: BM x BN per workgroup of WR x WC waves.  Two LDS stages of 128 bytes of k, filled by direct-to-LDS loads
-// two stages ahead; fragments are read one 16-k step ahead of the MFMAs that use them, across the stage border too, so
-// the one barrier of a stage sits between the last fragment reads of a stage and the MFMAs on them.
-// LDS stages in flight: two of 64 KB for the large tile; the small tile, whose stages are over in a fraction of a load's
-// latency, runs four
+// The tensors of the epilogue as buffers at the corner of a tile, addressed by row and by this lane's 8 columns.
+__device__ __forceinline__ u32x4 buf_load(const char* p, int bytes, int off) {
+#ifdef __HIP_DEVICE_COMPILE__
+    return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(__builtin_amdgcn_make_buffer_rsrc((void*)p, 0, bytes, 0x00020000), off, 0, 0));
+#else
+    return u32x4{0, 0, 0, 0};
+#endif
+}
+__device__ __forceinline__ void buf_store(char* p, int bytes, int off, u32x4 v) {
+#ifdef __HIP_DEVICE_COMPILE__
+    __builtin_amdgcn_raw_buffer_store_b128(v, __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, bytes, 0x00020000), off, 0, 0);
+#endif
+}
+struct Stream {
+    char* p;
+    int bytes, pitch, col;
+    // `present`: the tensor exists; pitches are at most MAX_PITCH, so offsets inside 256 rows stay below 2^31
+    __device__ __forceinline__ void init(const void* base, bool present, size_t ld, int es, size_t m0, int n0, int c) {
+        p = (char*)base + (m0 * ld + n0) * es;
+        bytes = present ? 0x7fffffff : 0;
+        pitch = (int)(ld * es);
+        col = c * es;
+    }
+    __device__ __forceinline__ int at(int row, bool ok) const { return ok ? row * pitch + col : -1; }
+    __device__ __forceinline__ void store_f32(int row, bool ok, const float (&v)[8]) const {
+        const int o = at(row, ok);
+        buf_store(p, bytes, o, __builtin_bit_cast(u32x4, f32x4{v[0], v[1], v[2], v[3]}));
+        buf_store(p, bytes, ok ? o + 16 : o, __builtin_bit_cast(u32x4, f32x4{v[4], v[5], v[6], v[7]}));
+    }
+    __device__ __forceinline__ void store_bf16(int row, bool ok, const float (&v)[8]) const {
+        bf16x8 r;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) r[j] = (bf16)v[j];
+        buf_store(p, bytes, at(row, ok), __builtin_bit_cast(u32x4, r));
+    }
+};
+template <typename T> struct Streams {
+    static constexpr bool B = sizeof(T) == 2;
+    static constexpr int NV = B ? 1 : 2;                           // 16-byte pieces of 8 elements
+    Stream res, pre32, out32, pre16, out16;
+    int act;
+    __device__ __forceinline__ Streams(const GemmArgs& a, int slice, int m0, int n0, int c) {
+        const bool slab = a.slab != nullptr;
+        res.init(a.e.res, !slab && a.e.res, a.e.res_ld, sizeof(T), m0, n0, c);
+        pre32.init(a.e.pre, !slab && a.e.pre && (!B || a.e.pre_f32), a.e.pre_ld, 4, m0, n0, c);
+        if (slab) out32.init(a.slab + (size_t)slice * a.M * a.N, true, a.N, 4, m0, n0, c);
+        else out32.init(a.e.out, !B || a.e.out_f32, a.e.out_ld, 4, m0, n0, c);
+        if constexpr (B) {
+            pre16.init(a.e.pre, !slab && a.e.pre && !a.e.pre_f32, a.e.pre_ld, 2, m0, n0, c);
+            out16.init(a.e.out, !slab && !a.e.out_f32, a.e.out_ld, 2, m0, n0, c);
+        }
+        act = slab ? CVG_ACT_NONE : a.e.act;
+    }
+    __device__ __forceinline__ void load(u32x4 (&q)[NV], int row, bool ok) const {
+        const int o = res.at(row, ok);
+        q[0] = buf_load(res.p, res.bytes, o);
+        if constexpr (!B) q[1] = buf_load(res.p, res.bytes, ok ? o + 16 : o);
+    }
+    __device__ __forceinline__ void emit(float (&v)[8], const float (&bias)[8], const u32x4 (&q)[NV], int row, bool ok) const {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] += bias[j];
+        pre32.store_f32(row, ok, v);
+        if constexpr (B) pre16.store_bf16(row, ok, v);
+        act_value8<!B>(v, act);
+        float r[8];
+        raw_f32(__builtin_bit_cast(Raw8<T>, q), r);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] += r[j];
+        out32.store_f32(row, ok, v);
+        if constexpr (B) out16.store_bf16(row, ok, v);
+    }
+};
+
+// Tile kernel: BM x BN per workgroup of 2 x 2 waves, 128 bytes of k per LDS stage.  Fragments are read one 16-k step ahead
+// of the MFMAs that use them, across the stage border too, so the one barrier of a stage sits between the last fragment
+// reads of a stage and the MFMAs on them.
+//   256 x 256 (bf16): a wave holds 128 x 128 sums, which needs the least LDS traffic per MFMA (8 fragments for 16 MFMAs; 64 x
+//     128 sums of eight waves need 6 for 8, and then the LDS is busy as long as the matrix units).  Its operands come by way
+//     of registers, a stage ahead of the LDS: fetching straight to LDS keeps the LDS busy for longer than writing 128 bytes
+//     a cycle does (8192 x 4096 x 4096 dw: staging alone takes 140 us, fragment reads alone 91, both together 221; the
+//     product with its 161 us of MFMAs 322).  dw 237 us (1160 TFLOP/s), dx 260, forward with f32 pre and residual 281.
+//   128 x 128 and 64 x 64: two workgroups share a CU and registers are short; direct-to-LDS loads.  Two LDS stages; the small
+//     tile, whose stages are over in a fraction of a load's latency, keeps four in flight.
 template <int BM> constexpr int ring() { return BM == 64 ? 4 : 2; }
 template <typename T, int BM, int BN, int WR, int WC> struct TileLds {
     static constexpr int STAGES = ring<BM>() * (BM + BN) * 128, EPI = WR * WC * 32 * (BN / WC * 4 + 16);
@@ -218,6 +310,7 @@ __device__ __forceinline__ void tile_body(const GemmArgs& a, int id, int slice, 
     typedef typename Elem<T>::frag frag;
     constexpr int BK = OA::BK, NS = BK / 16;
     constexpr int STAGE = OA::BYTES + OB::BYTES, D = ring<BM>();
+    constexpr bool REGS = BM == 256;
     constexpr int EP = WN * 4 + 16;                                // epilogue: 32 rows of the wave's columns, f32
     // workgroups go round-robin over the 8 dies, each with its own L2: give every die a run of neighbouring tiles, walked
     // in strips of 4 tile rows
@@ -239,6 +332,10 @@ __device__ __forceinline__ void tile_body(const GemmArgs& a, int id, int slice, 
     const bool whole = a.vec && n + 8 <= a.N;
     float bias[8];
     load_bias8(a.e, n, a.N, whole, bias);
+    if (a.slab) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) bias[j] = 0.f;
+    }
 
     OA oa;
     OB ob;
@@ -262,49 +359,49 @@ __device__ __forceinline__ void tile_body(const GemmArgs& a, int id, int slice, 
             for (int j = 0; j < TJ; ++j) far[i][j] = acc[i][j];
     }
     const int stages = (k_len + BK - 1) / BK, full = k_len / BK;
-    auto issue = [&](int st, int buf) {
+    constexpr int L = OA::NL + OB::NL, R = TI + TJ, MF = TI * TJ, H = MF > 1 ? MF / 2 : 1, HL = MF / 2;
+    // loads lo .. hi - 1 of a stage's L, straight to LDS
+    auto load = [&](auto whole_stage, int buf, int lo, int hi, int k_left) {
+        constexpr bool F = decltype(whole_stage)::value;
         char* base = lds + buf * STAGE;
-        if (st < full) {
-            oa.template issue<true>(base, 0);
-            ob.template issue<true>(base + OA::BYTES, 0);
-        } else {
-            oa.template issue<false>(base, k_len - st * BK);
-            ob.template issue<false>(base + OA::BYTES, k_len - st * BK);
+#pragma unroll
+        for (int i = 0; i < L; ++i) {
+            if (i < lo || i >= hi) continue;
+            if (i < OA::NL) oa.template load<F>(base, i, k_left);
+            else ob.template load<F>(base + OA::BYTES, i - OA::NL, k_left);
         }
     };
+    auto issue = [&](int st, int buf) {
+        if (st < full) load(Yes{}, buf, 0, L, 0);
+        else load(No{}, buf, 0, L, k_len - st * BK);
+    };
+    // fragments lo .. hi - 1 of the R of k-step s
     frag fa[2][TI], fb[2][TJ];
-    auto read = [&](int buf, int s, int into) {
+    auto read = [&](int buf, int s, int into, int lo, int hi) {
         const char* base = lds + buf * STAGE;
 #pragma unroll
-        for (int i = 0; i < TI; ++i) fa[into][i] = OA::frag(base, wm + i * 32, s, lane);
-#pragma unroll
-        for (int j = 0; j < TJ; ++j) fb[into][j] = OB::frag(base + OA::BYTES, wn + j * 32, s, lane);
+        for (int i = 0; i < R; ++i) {
+            if (i < lo || i >= hi) continue;
+            if (i < TI) fa[into][i] = OA::frag(base, wm + i * 32, s, lane);
+            else fb[into][i - TI] = OB::frag(base + OA::BYTES, wn + (i - TI) * 32, s, lane);
+        }
     };
-    constexpr bool MIX = TI * TJ >= 16;
-    auto multiply = [&](int from) {
-        if constexpr (MIX) {
+    // One 16-k step: behind MFMA q on fragment set `from` comes between(q).  An instruction that finds its unit's queue
+    // full holds up the wave's MFMAs too, so LDS reads (first half) and loads (second half) are dealt out evenly.  A single
+    // MFMA is over before the reads it would hide have arrived: they go first.
+    auto step = [&](int from, auto between) {
 #pragma unroll
-            for (int i = 0; i < TI; ++i)
-#pragma unroll
-                for (int j = 0; j < TJ; ++j) mma32(acc[i][j], fa[from][i], fb[from][j]);
-#pragma unroll
-            for (int g = 0; g < 8; ++g) {
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x020, 2, 0);
-            }
+        for (int q = 0; q < MF; ++q) {
+            if (MF == 1) between(q);
             __builtin_amdgcn_sched_barrier(0);
-            return;
+            mma32(acc[q / TJ][q % TJ], fa[from][q / TJ], fb[from][q % TJ]);
+            __builtin_amdgcn_sched_barrier(0);
+            if (MF > 1) between(q);
         }
         __builtin_amdgcn_sched_barrier(0);
-        __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-        for (int i = 0; i < TI; ++i)
-#pragma unroll
-            for (int j = 0; j < TJ; ++j) mma32(acc[i][j], fa[from][i], fb[from][j]);
-        __builtin_amdgcn_s_setprio(0);
-        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto deal_reads = [&](int q, int buf, int s, int into) {
+        if (q < H) read(buf, s, into, q * R / H, (q + 1) * R / H);
     };
     auto fold = [&](int st) {
         if constexpr (FOLD) {
@@ -319,55 +416,125 @@ __device__ __forceinline__ void tile_body(const GemmArgs& a, int id, int slice, 
         }
     };
     // The border between stage st and st + 1: this wave's reads of st have arrived and so has its part of st + 1; behind
-    // the barrier that holds for every wave, so st + 1 may be read and st overwritten.  While only whole stages are in
-    // flight the D - 2 stages behind st + 1 stay so; a partial one takes an unknown number of loads.
-    constexpr int L = OA::NL + OB::NL;
-    auto border = [&](auto steady) {
-        if constexpr (decltype(steady)::value) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"((D - 2) * L) : "memory");
+    // the barrier that holds for every wave, so st + 1 may be read and st overwritten.
+    constexpr int P = MF > 1 ? L / NS : L;                         // loads per step (short stages: all of them as early as can be)
+    static_assert(L % NS == 0, "tile");
+    int st = 0, buf = 0;
+    if constexpr (REGS) {
+        u32x4 hold[L];                                             // stage st + 1 (from step `NS - 1` of st on: st + 2)
+        auto fetch = [&](auto whole_stage, int lo, int hi, int k_left) {
+            constexpr bool F = decltype(whole_stage)::value;
+#pragma unroll
+            for (int i = 0; i < L; ++i) {
+                if (i < lo || i >= hi) continue;
+                if (i < OA::NL) hold[i] = oa.template fetch<F>(i, k_left);
+                else hold[i] = ob.template fetch<F>(i - OA::NL, k_left);
+            }
+        };
+        auto fetch_any = [&](int of, int lo, int hi) {
+            if (of < full) fetch(Yes{}, lo, hi, 0);
+            else if (of < stages) fetch(No{}, lo, hi, k_len - of * BK);
+        };
+        auto put = [&](int to, int lo, int hi) {
+            char* base = lds + to * STAGE;
+#pragma unroll
+            for (int i = 0; i < L; ++i) {
+                if (i < lo || i >= hi) continue;
+                if (i < OA::NL) oa.put(base, i, hold[i]);
+                else ob.put(base + OA::BYTES, i - OA::NL, hold[i]);
+            }
+        };
+        auto border = [&]() {
+            asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" : : : "memory");
+        };
+        fetch_any(0, 0, L);
+        put(0, 0, L);
+        fetch_any(1, 0, L);
+        border();
+        read(0, 0, 0, 0, R);
+        if (1 < stages) put(1, 0, P);
+        fetch_any(2, 0, P);
+        for (; st + 3 < full; ++st, buf ^= 1) {
+#pragma unroll
+            for (int s = 0; s < NS; ++s) {
+                const bool last = s == NS - 1;
+                if (last) border();
+                step(s & 1, [&](int q) {
+                    if (last) deal_reads(q, buf ^ 1, 0, 0);
+                    else deal_reads(q, buf, s + 1, (s + 1) & 1);
+                    const int n = last ? 0 : s + 1;
+#pragma unroll
+                    for (int i = 0; i < L; ++i)
+                        if (q >= HL && i >= n * P + (q - HL) * P / (MF - HL) && i < n * P + (q - HL + 1) * P / (MF - HL)) {
+                            put(last ? buf : buf ^ 1, i, i + 1);
+                            fetch(Yes{}, i, i + 1, 0);
+                        }
+                });
+            }
+        }
+        for (; st < stages; ++st, buf ^= 1) {
+#pragma unroll
+            for (int s = 0; s < NS - 1; ++s) {
+                step(s & 1, [&](int q) { deal_reads(q, buf, s + 1, (s + 1) & 1); });
+                if (st + 1 < stages) put(buf ^ 1, (s + 1) * P, (s + 2) * P);
+                fetch_any(st + 2, (s + 1) * P, (s + 2) * P);
+            }
+            border();
+            step((NS - 1) & 1, [&](int q) { if (st + 1 < stages) deal_reads(q, buf ^ 1, 0, 0); });
+            if (st + 2 < stages) put(buf, 0, P);
+            fetch_any(st + 3, 0, P);
+        }
+    } else {
+        // While only whole stages are in flight the D - 2 stages behind st + 1 stay so; a partial one takes an unknown
+        // number of loads.
+        auto border = [&](auto steady) {
+            if constexpr (decltype(steady)::value) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"((D - 2) * L) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" : : : "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" : : : "memory");
+        };
+        // a stage's loads are spread over NS steps, the first P in the last step of the stage whose place they take
+        for (int i = 0; i < D - 1 && i < stages; ++i) issue(i, i);
+        if (full > D) load(Yes{}, D - 1, 0, P, 0);
+        else if (D <= stages) issue(D - 1, D - 1);
+        if (full >= D) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"((D - 2) * L + P) : "memory");
         else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" : : : "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" : : : "memory");
-    };
-    for (int st = 0; st < D && st < stages; ++st) issue(st, st);
-    if (full >= D) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"((D - 1) * L) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" : : : "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" : : : "memory");
-    read(0, 0, 0);
-    int st = 0, buf = 0;
-    for (; st + D < full; ++st) {
-        const int after = buf + 1 == D ? 0 : buf + 1;
+        read(0, 0, 0, 0, R);
+        int before = D - 1;
+        for (; st + D < full; ++st) {
+            const int after = buf + 1 == D ? 0 : buf + 1;
 #pragma unroll
-        for (int s = 0; s < NS; ++s) {
-            if (s < NS - 1) {
-                read(buf, s + 1, (s + 1) & 1);
-            } else {
-                border(Yes{});
-                read(after, 0, (s + 1) & 1);
-                char* base = lds + buf * STAGE;
-                oa.template issue<true>(base, 0);
-                ob.template issue<true>(base + OA::BYTES, 0);
+            for (int s = 0; s < NS; ++s) {
+                const bool last = s == NS - 1;
+                if (last) border(Yes{});
+                step(s & 1, [&](int q) {
+                    if (last) deal_reads(q, after, 0, 0);
+                    else deal_reads(q, buf, s + 1, (s + 1) & 1);
+                    const int n = last ? 0 : s + 1;
+                    if (q >= HL) load(Yes{}, last ? buf : before, n * P + (q - HL) * P / (MF - HL), n * P + (q - HL + 1) * P / (MF - HL), 0);
+                });
             }
-            multiply(s & 1);
+            fold(st);
+            before = buf;
+            buf = after;
         }
-        fold(st);
-        buf = after;
-    }
-    for (; st < stages; ++st) {
-        const int after = buf + 1 == D ? 0 : buf + 1;
+        if (st > 0) load(Yes{}, before, P, L, 0);
+        for (; st < stages; ++st) {
+            const int after = buf + 1 == D ? 0 : buf + 1;
 #pragma unroll
-        for (int s = 0; s < NS; ++s) {
-            if (s < NS - 1) {
-                read(buf, s + 1, (s + 1) & 1);
-            } else if (st + 1 < stages) {
+            for (int s = 0; s < NS - 1; ++s) step(s & 1, [&](int q) { deal_reads(q, buf, s + 1, (s + 1) & 1); });
+            if (st + 1 < stages) {
                 border(No{});
-                read(after, 0, (s + 1) & 1);
                 if (st + D < stages) issue(st + D, buf);
             }
-            multiply(s & 1);
+            step((NS - 1) & 1, [&](int q) { if (st + 1 < stages) deal_reads(q, after, 0, 0); });
+            fold(st);
+            buf = after;
         }
-        fold(st);
-        buf = after;
     }
     if constexpr (FOLD) {
 #pragma unroll
@@ -381,21 +548,55 @@ __device__ __forceinline__ void tile_body(const GemmArgs& a, int id, int slice, 
     __syncthreads();
     char* ep = lds + wave * 32 * EP;
     const int l31 = lane & 31, h = lane >> 5;
-    const bool has_res = !a.slab && a.e.res;
     constexpr int PG = PASSES < 4 ? PASSES : 4;                    // passes whose residual is loaded together
-#pragma unroll
-    for (int i = 0; i < TI; ++i) {
+    auto to_lds = [&](int i) {                                     // (the region is this wave's own: its accesses complete in order)
 #pragma unroll
         for (int j = 0; j < TJ; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e)
                 *(float*)(ep + ((e & 3) + 8 * (e >> 2) + 4 * h) * EP + (j * 32 + l31) * 4) = acc[i][j][e];
-        // (the region is this wave's own: its LDS accesses complete in order)
+    };
+    auto from_lds = [&](int pass, float (&v)[8]) { load8<float>((const float*)(ep + (pass * RPP + rl) * EP + cl * 4), v); };
+    if (a.fast) {
+        // No branch around a memory access: a tensor that is not there has a descriptor of no bytes, a row or column outside
+        // the matrix an offset beyond every descriptor.  So the number of accesses between a residual's load and its use is
+        // known, and waiting for it waits for no store.
+        const Streams<T> io(a, slice, m0, n0, wn + cl);
+        u32x4 next[PG][Streams<T>::NV], q[PG][Streams<T>::NV];
+        const int row0 = wm + rl, rows = n < a.N ? a.M - m0 : 0;
+#pragma unroll
+        for (int r = 0; r < PG; ++r) io.load(next[r], row0 + r * RPP, row0 + r * RPP < rows);
+#pragma unroll
+        for (int i = 0; i < TI; ++i) {
+            to_lds(i);
+#pragma unroll 1
+            for (int r0 = 0; r0 < PASSES; r0 += PG) {
+                const int row = row0 + i * 32 + r0 * RPP;
+#pragma unroll
+                for (int r = 0; r < PG; ++r) {
+#pragma unroll
+                    for (int k = 0; k < Streams<T>::NV; ++k) q[r][k] = next[r][k];
+                    const int rn = row + (PG + r) * RPP;           // (PASSES RPP is 32: behind a block's last group the next block's first)
+                    io.load(next[r], rn, rn < rows && rn < wm + WM);
+                }
+#pragma unroll
+                for (int r = 0; r < PG; ++r) {
+                    float v[8];
+                    from_lds(r0 + r, v);
+                    io.emit(v, bias, q[r], row + r * RPP, row + r * RPP < rows);
+                }
+            }
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < TI; ++i) {
+        to_lds(i);
 #pragma unroll 1
         for (int r0 = 0; r0 < PASSES; r0 += PG) {
             const int mb = m0 + wm + i * 32 + r0 * RPP + rl;
             float q[PG][8];
-            if (has_res && n < a.N) {
+            if (!a.slab && a.e.res && n < a.N) {
 #pragma unroll
                 for (int r = 0; r < PG; ++r) load_res8<T>(a.e, min(mb + r * RPP, a.M - 1), n, a.N, whole, q[r]);
             }
@@ -403,14 +604,13 @@ __device__ __forceinline__ void tile_body(const GemmArgs& a, int id, int slice, 
             for (int r = 0; r < PG; ++r) {
                 const int m = mb + r * RPP;
                 float v[8];
-                load8<float>((const float*)(ep + ((r0 + r) * RPP + rl) * EP + cl * 4), v);
+                from_lds(r0 + r, v);
                 if (m >= a.M || n >= a.N) continue;
                 if (a.slab) {
                     float* o = a.slab + ((size_t)slice * a.M + m) * a.N + n;
-                    if (n + 8 <= a.N && (a.N & 3) == 0) store8<float>(o, v);
-                    else
-                        for (int j = 0; j < 8; ++j)
-                            if (n + j < a.N) o[j] = v[j];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (n + j < a.N) o[j] = v[j];
                 } else {
                     emit8<T>(a.e, m, n, a.N, whole, v, bias, q[r]);
                 }
@@ -823,6 +1023,9 @@ GemmArgs gemm_args(const Rows& A, bool acol, const Rows& B, bool bcol, int64_t M
     a.tiles_n = ceil_div(N, sh.bn);
     a.k_split = t.k_split;
     a.slab = t.splits > 1 ? (float*)ws : nullptr;
+    a.fast = N % 8 == 0 && (a.slab ? (size_t)N * 4 <= MAX_PITCH
+                                   : a.vec && e.out_ld * oes <= MAX_PITCH && (!e.pre || e.pre_ld * pes <= MAX_PITCH) &&
+                                         (!e.res || e.res_ld * sizeof(T) <= MAX_PITCH));
     ws += slab_of(t, M, N);
     return a;
 }
@@ -849,8 +1052,7 @@ template <typename T>
 int multiply(GemmArgs& a, bool acol, bool bcol, const Tile& t, hipStream_t s) {
     if (t.cfg == 0) {
         if constexpr (sizeof(T) == 2) {
-            if (getenv("LIN_4W")) launch_tile<T, 256, 256, 2, 2>(a, acol, bcol, t.splits, s);
-            else launch_tile<T, 256, 256, 2, 4>(a, acol, bcol, t.splits, s);
+            launch_tile<T, 256, 256, 2, 2>(a, acol, bcol, t.splits, s);
         }
     } else if (t.cfg == 1) {
         launch_tile<T, 128, 128, 2, 2>(a, acol, bcol, t.splits, s);

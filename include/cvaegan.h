@@ -462,7 +462,7 @@ enum { CVG_ACT_NONE = 0, CVG_ACT_LRELU = 1 /* slope 0.2 */, CVG_ACT_SILU = 2, CV
  *   y = act( gamma[c] * (x - mean) * rstd + beta[c] [+ res] ),  mean and rstd = 1 / sqrt(var + eps) (biased
  * variance) over the HW pixels and C / G channels of one sample and group.
  * Tensors are [B * HW] pixel rows of C channels at the pitches of the descriptor (elements, 0 = C).  C is a multiple
- * of 8, G divides C, the least common multiple of 8 and C / G is at most 2048; pointers are 16-byte aligned and
+ * of 8, G divides C, the least common multiple of 8 and C / G is at most 4096; pointers are 16-byte aligned and
  * pitches multiples of 16 bytes.  B may be 0.
  * stats f32 [2][B][G] = mean, rstd: written by the forward call, read by the backward call.
  * y may be x or res itself; other overlaps of an output with an input are not supported.                     */
