@@ -374,7 +374,7 @@ extern "C" int cvg_distill_topk(const cvg_distill_desc* d, const void* logits, c
     CVG_CHECK(d, "distill_topk: null descriptor");
     CVG_CHECK(d->dtype == CVG_F32 || d->dtype == CVG_BF16, "distill_topk: dtype %d", d->dtype);
     CVG_CHECK(d->R >= 0 && d->V >= 1, "distill_topk: R %d, V %d", d->R, d->V);
-    CVG_CHECK(d->V <= 0x7ffffff0, "distill_topk: V %d", d->V);
+    CVG_CHECK(d->R <= 0x7fff0000 && d->V <= 0x7ffffff0, "distill_topk: R %d, V %d", d->R, d->V);   // (row loops step past the end)
     CVG_CHECK(d->top >= 1 && d->top <= MAX_TOP, "distill_topk: %d teacher entries (1..%d)", d->top, MAX_TOP);
     CVG_CHECK(d->temperature > 0.f && d->temperature < INFINITY, "distill_topk: temperature %g", (double)d->temperature);
     CVG_CHECK((d->logits_ld == 0 || d->logits_ld >= d->V) && (d->dlogits_ld == 0 || d->dlogits_ld >= d->V) &&

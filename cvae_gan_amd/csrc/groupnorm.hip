@@ -517,7 +517,7 @@ int check(const cvg_gn_desc* d, const char* who) {
     CVG_CHECK(d->C % d->G == 0, "%s: %d groups do not divide %d channels", who, d->G, d->C);
     const int cg = d->C / d->G;
     CVG_CHECK((int64_t)cg / gcd(cg, 8) * 8 <= 4096, "%s: groups of %d channels are too wide", who, cg);
-    CVG_CHECK((int64_t)d->B * d->HW <= 0x7fffffff, "%s: %lld pixel rows", who, (long long)d->B * d->HW);
+    CVG_CHECK((int64_t)d->B * d->HW <= 0x7fff0000, "%s: %lld pixel rows", who, (long long)d->B * d->HW);   // (row loops step past the end)
     CVG_CHECK(act_known(d->act), "%s: activation %d", who, d->act);
     CVG_CHECK(d->eps >= 0.f, "%s: eps %g", who, (double)d->eps);
     const int per16 = d->dtype == CVG_BF16 ? 8 : 4;
@@ -587,6 +587,7 @@ void fill(GnArgs& a, const cvg_gn_desc* d, const Plan& p) {
     a.cg = make_fastdiv(d->C / d->G); a.nvd = make_fastdiv(p.nv); a.tiled = make_fastdiv(p.tiles); a.slabd = make_fastdiv(p.nslab);
 }
 
+bool launchable(const cvg_gn_desc* d, const Plan& p) { return (int64_t)d->B * p.nslab * p.tiles * p.threads < (int64_t)1 << 32; }
 size_t ws_need(const cvg_gn_desc* d, const Plan& p, bool backward) {
     if (backward) return (size_t)d->B * p.tiles * 2 * d->C * 4;
     return p.tiles > 1 ? (size_t)d->B * d->G * p.tiles * 2 * 4 : 0;
@@ -652,9 +653,11 @@ int cvg_gn_act_fwd(const cvg_gn_desc* d, const void* x, const void* res, void* y
     CVG_CHECK(x && y, "gn_act_fwd: null tensor");
     CVG_CHECK(aligned16(x) && aligned16(res) && aligned16(y), "gn_act_fwd: tensors have to start at 16-byte borders");
     const Plan p = plan(d, false, res != nullptr);
-    CVG_CHECK((int64_t)d->B * p.nslab * p.tiles <= 0x7fffffff, "gn_act_fwd: too many tiles");
+    CVG_CHECK(launchable(d, p), "gn_act_fwd: too many tiles");
     const size_t need = ws_need(d, p, false);
     CVG_CHECK(need == 0 || (ws && ws_bytes >= need && ((uintptr_t)ws & 3) == 0), "gn_act_fwd: workspace of %zu bytes, need %zu", ws_bytes, need);
+    const int x_ld = d->x_ld ? d->x_ld : d->C, res_ld = d->res_ld ? d->res_ld : d->C, y_ld = d->y_ld ? d->y_ld : d->C;
+    CVG_CHECK((y != x || y_ld == x_ld) && (y != res || y_ld == res_ld), "gn_act_fwd: in place with different pitches");
     GnArgs a{};
     fill(a, d, p);
     a.x = x; a.res = res; a.y = y; a.stats = stats; a.gamma = gamma; a.beta = beta; a.part = (float*)ws;
@@ -673,9 +676,13 @@ int cvg_gn_act_bwd(const cvg_gn_desc* d, const void* dy, const void* x, const vo
     CVG_CHECK(aligned16(x) && aligned16(res) && aligned16(dy) && aligned16(dx) && aligned16(dres),
               "gn_act_bwd: tensors have to start at 16-byte borders");
     const Plan p = plan(d, true, res != nullptr);
-    CVG_CHECK((int64_t)d->B * p.nslab * p.tiles <= 0x7fffffff, "gn_act_bwd: too many tiles");
+    CVG_CHECK(launchable(d, p), "gn_act_bwd: too many tiles");
     const size_t need = ws_need(d, p, true);
     CVG_CHECK(need == 0 || (ws && ws_bytes >= need && ((uintptr_t)ws & 3) == 0), "gn_act_bwd: workspace of %zu bytes, need %zu", ws_bytes, need);
+    const int dy_ld = d->y_ld ? d->y_ld : d->C, dx_ld = d->dx_ld ? d->dx_ld : d->C, dres_ld = d->dres_ld ? d->dres_ld : d->C;
+    CVG_CHECK(!dy || ((dx != dy || dx_ld == dy_ld) && (dres != dy || dres_ld == dy_ld)), "gn_act_bwd: in place with different pitches");
+    CVG_CHECK(!dx || (dx != dres && dx != x && dx != res && (!dres || (dres != x && dres != res))),
+              "gn_act_bwd: a gradient over another tensor");
     GnArgs a{};
     fill(a, d, p);
     a.x = x; a.res = res; a.dy = dy; a.dx = dx; a.dres = dres; a.stats = (float*)stats; a.gamma = gamma; a.beta = beta;

@@ -296,15 +296,15 @@ template <typename T> struct Streams {
 //   128 x 128 and 64 x 64: two workgroups share a CU and registers are short; direct-to-LDS loads.  Two LDS stages; the small
 //     tile, whose stages are over in a fraction of a load's latency, keeps four in flight.
 template <int BM> constexpr int ring() { return BM == 64 ? 4 : 2; }
-template <typename T, int BM, int BN, int WR, int WC> struct TileLds {
-    static constexpr int STAGES = ring<BM>() * (BM + BN) * 128, EPI = WR * WC * 32 * (BN / WC * 4 + 16);
+template <typename T, int BM, int BN> struct TileLds {
+    static constexpr int STAGES = ring<BM>() * (BM + BN) * 128, EPI = 4 * 32 * (BN / 2 * 4 + 16);
     static constexpr int BYTES = STAGES > EPI ? STAGES : EPI;
 };
 struct Yes { static constexpr bool value = true; };
 struct No { static constexpr bool value = false; };
-template <typename T, int BM, int BN, int WR, int WC, bool ACOL, bool BCOL>
+template <typename T, int BM, int BN, bool ACOL, bool BCOL>
 __device__ __forceinline__ void tile_body(const GemmArgs& a, int id, int slice, char* lds) {
-    constexpr int NW = WR * WC, WM = BM / WR, WN = BN / WC, TI = WM / 32, TJ = WN / 32;
+    constexpr int NW = 4, WM = BM / 2, WN = BN / 2, TI = WM / 32, TJ = WN / 32;
     typedef Operand<T, BM, NW, ACOL> OA;
     typedef Operand<T, BN, NW, BCOL> OB;
     typedef typename Elem<T>::frag frag;
@@ -324,7 +324,7 @@ __device__ __forceinline__ void tile_body(const GemmArgs& a, int id, int slice, 
     const int m0 = (strip * 4 + in % h_strip) * BM, n0 = (in / h_strip) * BN;
     const int k0 = slice * a.k_split, k_len = min(a.K - k0, a.k_split);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int wm = (wave / WC) * WM, wn = (wave % WC) * WN;
+    const int wm = (wave >> 1) * WM, wn = (wave & 1) * WN;
 
     // this lane's columns in the epilogue; their bias is on its way while the products are taken
     constexpr int LPR = WN / 8, RPP = 64 / LPR, PASSES = 32 / RPP;      // lanes per row, rows per pass
@@ -619,10 +619,10 @@ __device__ __forceinline__ void tile_body(const GemmArgs& a, int id, int slice, 
     }
 }
 
-template <typename T, int BM, int BN, int WR, int WC, bool ACOL, bool BCOL>
-__global__ void __launch_bounds__(WR * WC * 64) gemm_tile(const GemmArgs a) {
-    __shared__ __attribute__((aligned(1024))) char lds[TileLds<T, BM, BN, WR, WC>::BYTES];
-    tile_body<T, BM, BN, WR, WC, ACOL, BCOL>(a, blockIdx.x, blockIdx.y, lds);
+template <typename T, int BM, int BN, bool ACOL, bool BCOL>
+__global__ void __launch_bounds__(256) gemm_tile(const GemmArgs a) {
+    __shared__ __attribute__((aligned(1024))) char lds[TileLds<T, BM, BN>::BYTES];
+    tile_body<T, BM, BN, ACOL, BCOL>(a, blockIdx.x, blockIdx.y, lds);
 }
 
 // ---- few rows: M <= 16 MT ------------------------------------------------------------------------------------
@@ -721,17 +721,17 @@ struct SumArgs { const float* part; float* out; int P, N; };
 
 // Both gradients of a layer in one launch: neither waits for the other, small ones do not fill the chip alone, and a
 // launch costs as much as they do.  The blocks behind the two products finish the bias gradient.
-template <typename T, int BM, int BN, int WR, int WC>
-__global__ void __launch_bounds__(WR * WC * 64) gemm_pair(const GemmArgs dx, const GemmArgs dw, int blocks_dx, int blocks_dw, const SumArgs db) {
-    __shared__ __attribute__((aligned(1024))) char lds[TileLds<T, BM, BN, WR, WC>::BYTES];
+template <typename T, int BM, int BN>
+__global__ void __launch_bounds__(256) gemm_pair(const GemmArgs dx, const GemmArgs dw, int blocks_dx, int blocks_dw, const SumArgs db) {
+    __shared__ __attribute__((aligned(1024))) char lds[TileLds<T, BM, BN>::BYTES];
     int blk = blockIdx.x;
     if (blk < blocks_dx) {
         const int nt = dx.tiles_m * dx.tiles_n, slice = blk / nt;
-        tile_body<T, BM, BN, WR, WC, false, true>(dx, blk - slice * nt, slice, lds);
+        tile_body<T, BM, BN, false, true>(dx, blk - slice * nt, slice, lds);
     } else if (blk < blocks_dx + blocks_dw) {
         blk -= blocks_dx;
         const int nt = dw.tiles_m * dw.tiles_n, slice = blk / nt;
-        tile_body<T, BM, BN, WR, WC, true, true>(dw, blk - slice * nt, slice, lds);
+        tile_body<T, BM, BN, true, true>(dw, blk - slice * nt, slice, lds);
     } else {
         sum_rows_body(db.part, db.P, db.N, db.out, blk - blocks_dx - blocks_dw, (float (*)[32])lds);
     }
@@ -899,10 +899,10 @@ __global__ void __launch_bounds__(256) prepare(const DzJob dz, const PadJob p0, 
 }
 
 __global__ void __launch_bounds__(256) zero_rows(char* out, size_t pitch, int rows, int width, int es) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= (int64_t)rows * width) return;
-    char* q = out + (size_t)(i / width) * pitch + (size_t)(i % width) * es;
-    if (es == 4) *(float*)q = 0.f; else *(bf16*)q = (bf16)0.f;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < (int64_t)rows * width; i += (int64_t)gridDim.x * 256) {
+        char* q = out + (size_t)(i / width) * pitch + (size_t)(i % width) * es;
+        if (es == 4) *(float*)q = 0.f; else *(bf16*)q = (bf16)0.f;
+    }
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------
@@ -928,17 +928,21 @@ int check(const cvg_linear_desc* d, const char* who) {
     for (int i = 0; i < 8; ++i)
         CVG_CHECK(ld[i] == 0 || ld[i] >= (i < 4 ? d->K : d->N), "%s: pitch %d below the row length %d", who, ld[i], i < 4 ? d->K : d->N);
     const int64_t m = ceil_div(d->M, 64), n = ceil_div(d->N, 64), k = ceil_div(d->K, 64);
-    CVG_CHECK(m * n <= 0x1000000 && m * k <= 0x1000000 && n * k <= 0x1000000, "%s: too many tiles", who);
+    CVG_CHECK(m * n < 0x400000 && m * k < 0x400000 && n * k < 0x400000, "%s: too many tiles", who);   // (a launch has fewer than 2^32 threads)
     return 0;
 }
 
 // Tile and number of K ranges for one product.  The estimate is in MFMA cycles of one CU: a stage (128 bytes of k) of a
 // BM x BN tile takes `mfma` cycles of its matrix units, never less than the load latency a two-stage pipeline leaves
 // exposed; workgroups beyond one round queue up; K ranges add their f32 slabs (written and read once at ~2000 bytes per
-// cycle chip-wide) and a launch.
+// cycle chip-wide) and a launch.  Forward bf16, us by 256 x 256 / 128 x 128 / 64 x 64 tiles:
+//   4096 x 4096 x 4096  116 / 131 / 204    2048 x 2048 x 2048  46 / 28 / 29    8192 x 1024 x 1024  35 / 23 / 31
+//   3000 x 3000 x 1000   39 /  41 /  45     512 x 4096 x 4096  45 / 35 / 27     550 x 8192 x  528  26 / 15 / 18
+// f32, whose MFMAs take eight times as long and need no more bytes, always takes 64 x 64: 128 x 128 measured 1114 against
+// 1024 us at 4096 x 4096 x 4096, 217 against 160 at 3000 x 3000 x 1000.
 struct Tile { int cfg, splits, k_split; double t; };
 struct TileShape { int bm, bn, occ; double mfma; };
-const TileShape TILES[2][3] = {{{0, 0, 0, 0}, {128, 128, 2, 4096 / .85}, {64, 64, 2, 1024 / .7}},
+const TileShape TILES[2][3] = {{{0, 0, 0, 0}, {0, 0, 0, 0}, {64, 64, 2, 1024 / .7}},
                                {{256, 256, 1, 2048 / .8}, {128, 128, 2, 512 / .6}, {64, 64, 2, 128 / .4}}};
 Tile choose_split(int dtype, int c, int64_t M, int64_t N, int64_t K) {
     const TileShape& sh = TILES[dtype == CVG_BF16][c];
@@ -963,7 +967,7 @@ Tile choose_split(int dtype, int c, int64_t M, int64_t N, int64_t K) {
 }
 Tile choose(int dtype, int64_t M, int64_t N, int64_t K) {
     Tile best{2, 1, 0, 1e301};
-    for (int c = dtype == CVG_BF16 ? 0 : 1; c < 3; ++c) {
+    for (int c = dtype == CVG_BF16 ? 0 : 2; c < 3; ++c) {
         const Tile t = choose_split(dtype, c, M, N, K);
         if (t.t < best.t) best = t;
     }
@@ -983,12 +987,12 @@ PairPlan choose_pair(const cvg_linear_desc* d) {
 }
 size_t slab_of(const Tile& t, int64_t M, int64_t N) { return t.splits > 1 ? round_up((size_t)t.splits * M * N * 4, 256) : 0; }
 
-template <typename T, int BM, int BN, int WR, int WC>
+template <typename T, int BM, int BN>
 void launch_tile(GemmArgs& a, bool acol, bool bcol, int splits, hipStream_t s) {
     const dim3 grid(a.tiles_m * a.tiles_n, splits);
-    if (!acol && !bcol) gemm_tile<T, BM, BN, WR, WC, false, false><<<grid, WR * WC * 64, 0, s>>>(a);
-    else if (!acol) gemm_tile<T, BM, BN, WR, WC, false, true><<<grid, WR * WC * 64, 0, s>>>(a);
-    else gemm_tile<T, BM, BN, WR, WC, true, true><<<grid, WR * WC * 64, 0, s>>>(a);
+    if (!acol && !bcol) gemm_tile<T, BM, BN, false, false><<<grid, 256, 0, s>>>(a);
+    else if (!acol) gemm_tile<T, BM, BN, false, true><<<grid, 256, 0, s>>>(a);
+    else gemm_tile<T, BM, BN, true, true><<<grid, 256, 0, s>>>(a);
 }
 
 // An operand as the caller holds it: `rows` rows of `width` elements.
@@ -1050,15 +1054,11 @@ int sum_slabs(const SlabJob& one, const SlabJob& two, hipStream_t s) {
 }
 template <typename T>
 int multiply(GemmArgs& a, bool acol, bool bcol, const Tile& t, hipStream_t s) {
-    if (t.cfg == 0) {
-        if constexpr (sizeof(T) == 2) {
-            launch_tile<T, 256, 256, 2, 2>(a, acol, bcol, t.splits, s);
-        }
-    } else if (t.cfg == 1) {
-        launch_tile<T, 128, 128, 2, 2>(a, acol, bcol, t.splits, s);
-    } else {
-        launch_tile<T, 64, 64, 2, 2>(a, acol, bcol, t.splits, s);
+    if constexpr (sizeof(T) == 2) {
+        if (t.cfg == 0) launch_tile<T, 256, 256>(a, acol, bcol, t.splits, s);
+        else if (t.cfg == 1) launch_tile<T, 128, 128>(a, acol, bcol, t.splits, s);
     }
+    if (t.cfg == 2) launch_tile<T, 64, 64>(a, acol, bcol, t.splits, s);
     CVG_LAUNCH_CHECK();
     return sum_slabs<T>(slab_job<T>(a, t), SlabJob{}, s);
 }
@@ -1160,8 +1160,10 @@ int backward(const cvg_linear_desc* d, const void* dy, const void* x, const void
     const int sum_blocks = dbias ? ceil_div(d->N, 32) : 0;
     if (plan.together && products) {
         const int bx = dx ? ax.tiles_m * ax.tiles_n * plan.dx.splits : 0, bw = dw ? aw.tiles_m * aw.tiles_n * plan.dw.splits : 0;
-        if (plan.dx.cfg == 1) gemm_pair<T, 128, 128, 2, 2><<<bx + bw + sum_blocks, 256, 0, s>>>(ax, aw, bx, bw, sum);
-        else gemm_pair<T, 64, 64, 2, 2><<<bx + bw + sum_blocks, 256, 0, s>>>(ax, aw, bx, bw, sum);
+        if constexpr (sizeof(T) == 2) {
+            if (plan.dx.cfg == 1) gemm_pair<T, 128, 128><<<bx + bw + sum_blocks, 256, 0, s>>>(ax, aw, bx, bw, sum);
+        }
+        if (plan.dx.cfg == 2) gemm_pair<T, 64, 64><<<bx + bw + sum_blocks, 256, 0, s>>>(ax, aw, bx, bw, sum);
         CVG_LAUNCH_CHECK();
         return sum_slabs<T>(dx ? slab_job<T>(ax, plan.dx) : SlabJob{}, dw ? slab_job<T>(aw, plan.dw) : SlabJob{}, s);
     }
@@ -1177,7 +1179,8 @@ int backward(const cvg_linear_desc* d, const void* dy, const void* x, const void
 // no rows: the sums are zero
 int backward_empty(const cvg_linear_desc* d, void* dw, float* dbias, hipStream_t s) {
     const int es = d->dw_dtype == CVG_F32 ? 4 : 2;
-    if (dw) zero_rows<<<ceil_div((int64_t)d->N * d->K, 256), 256, 0, s>>>((char*)dw, ld_of(d->dw_ld, d->K) * es, d->N, d->K, es);
+    const int64_t dw_blocks = ((int64_t)d->N * d->K + 255) / 256;
+    if (dw) zero_rows<<<(int)(dw_blocks < 65536 ? dw_blocks : 65536), 256, 0, s>>>((char*)dw, ld_of(d->dw_ld, d->K) * es, d->N, d->K, es);
     if (dbias) zero_rows<<<ceil_div(d->N, 256), 256, 0, s>>>((char*)dbias, 0, 1, d->N, 4);
     CVG_LAUNCH_CHECK();
     return 0;
@@ -1203,6 +1206,8 @@ int cvg_linear_act_fwd(const cvg_linear_desc* d, const void* x, const void* w, c
     CVG_CHECK((uintptr_t)pre % es_of(d->pre_dtype) == 0 && (uintptr_t)bias % 4 == 0, "linear_act_fwd: misaligned tensor");
     const size_t need = fwd_ws(d);
     CVG_CHECK(need == 0 || (ws && ws_bytes >= need && aligned16(ws)), "linear_act_fwd: workspace of %zu bytes, need %zu", ws_bytes, need);
+    CVG_CHECK(y != x && y != w && y != pre && (!pre || (pre != x && pre != w && pre != res)), "linear_act_fwd: an output over another tensor");
+    CVG_CHECK(y != res || ld_of(d->res_ld, d->N) == ld_of(d->y_ld, d->N), "linear_act_fwd: in place with different pitches");
     hipStream_t st = (hipStream_t)s;
     return d->dtype == CVG_BF16 ? forward<bf16>(d, x, w, bias, res, y, pre, (char*)ws, st)
                                 : forward<float>(d, x, w, bias, res, y, pre, (char*)ws, st);
@@ -1222,6 +1227,8 @@ int cvg_linear_act_bwd(const cvg_linear_desc* d, const void* dy, const void* x, 
     CVG_CHECK((uintptr_t)dw % es_of(d->dw_dtype) == 0, "linear_act_bwd: misaligned dw");
     const size_t need = bwd_ws(d);
     CVG_CHECK(need == 0 || (ws && ws_bytes >= need && aligned16(ws)), "linear_act_bwd: workspace of %zu bytes, need %zu", ws_bytes, need);
+    const void* outs[3] = {dx, dw, dbias};
+    for (const void* o : outs) CVG_CHECK(!o || (o != dy && o != x && o != w && o != pre), "linear_act_bwd: a gradient over another tensor");
     hipStream_t st = (hipStream_t)s;
     if (d->M == 0) return backward_empty(d, dw, dbias, st);
     char* w0 = (char*)ws;

@@ -463,9 +463,9 @@ enum { CVG_ACT_NONE = 0, CVG_ACT_LRELU = 1 /* slope 0.2 */, CVG_ACT_SILU = 2, CV
  * variance) over the HW pixels and C / G channels of one sample and group.
  * Tensors are [B * HW] pixel rows of C channels at the pitches of the descriptor (elements, 0 = C).  C is a multiple
  * of 8, G divides C, the least common multiple of 8 and C / G is at most 4096; pointers are 16-byte aligned and
- * pitches multiples of 16 bytes.  B may be 0.
+ * pitches multiples of 16 bytes.  B may be 0; B * HW is at most 0x7fff0000.
  * stats f32 [2][B][G] = mean, rstd: written by the forward call, read by the backward call.
- * y may be x or res itself; other overlaps of an output with an input are not supported.                     */
+ * y may be x or res itself, at the same pitch; other overlaps of an output with an input are not supported.  */
 typedef struct cvg_gn_desc {
     int32_t dtype, B, HW, C, G, act;
     int32_t x_ld, res_ld, y_ld;              /* forward: x, res, y; backward: x, res, dy                        */
@@ -478,7 +478,7 @@ int cvg_gn_act_fwd(const cvg_gn_desc* d, const void* x, const void* res, void* y
 /* g = dy * act'(pre), pre recomputed from x, stats and res (NULL as in the forward call);
  *   dx = rstd * (gamma g - mean_group(gamma g) - xhat mean_group(gamma g xhat)),  dres = g (may be NULL),
  *   dgamma[c] = sum g xhat, dbeta[c] = sum g over samples and pixels (f32, overwritten).
- * dx or dres may be dy itself.                                                                                */
+ * dx or dres may be dy itself, at the same pitch.                                                             */
 int cvg_gn_act_bwd(const cvg_gn_desc* d, const void* dy, const void* x, const void* res, void* dx, void* dres,
                    const float* stats, const float* gamma, const float* beta, float* dgamma, float* dbeta,
                    void* ws, size_t ws_bytes, cvg_stream s);
@@ -487,8 +487,9 @@ int cvg_gn_act_bwd(const cvg_gn_desc* d, const void* dy, const void* x, const vo
  *   x [M][K], w [N][K] (the layout of nn.Linear, unpacked), y / res / pre [M][N] in d->dtype, bias f32 [N] or NULL;
  *   pre (may be NULL) receives the argument of the activation for the backward call, in d->pre_dtype: f32 keeps its
  *   derivative, and with it dbias, at f32 accuracy; the type of the data halves what the backward call reads.
- * Row pitches in elements (0 = dense); any M >= 0, N and K from 1 to 2000000, and any element-aligned pointer; rows of whole 16 bytes
- * at 16-byte aligned addresses take the fast paths.  y may be res itself.
+ * Row pitches in elements (0 = dense); any M >= 0, N and K from 1 to 2000000, less than 0x400000 blocks of 64 x 64 in
+ * each of x, w and y, and any element-aligned pointer; rows of whole 16 bytes at 16-byte aligned addresses take the fast
+ * paths.  y may be res itself, at the same pitch; other overlaps of an output with an input are not supported.
  * Products are exact, sums f32; f32 data uses exact-f32 MFMA.                                                  */
 typedef struct cvg_linear_desc {
     int32_t dtype, M, N, K, act;
@@ -511,7 +512,7 @@ int cvg_linear_act_bwd(const cvg_linear_desc* d, const void* dy, const void* x, 
  * An entry whose index lies outside [0, V) is absent (rows with fewer than `top` teacher entries); an index may
  * appear twice.  A row of weight 0, or without an entry of finite value or NaN, has loss and gradient 0 whatever it
  * holds.  row_weight f32 [R] or NULL (ones); row_loss f32 [R]; dlogits (dtype, pitch dlogits_ld) or NULL;
- * dlogits may be logits itself.  R >= 0, 1 <= V, 1 <= top <= 1024, T > 0; pitches 0 = dense.                    */
+ * dlogits may be logits itself, at the same pitch.  0 <= R <= 0x7fff0000, 1 <= V <= 0x7ffffff0, 1 <= top <= 1024, T > 0; pitches 0 = dense.                    */
 typedef struct cvg_distill_desc {
     int32_t dtype, R, V, top;
     int32_t logits_ld, dlogits_ld, top_ld;

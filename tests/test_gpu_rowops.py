@@ -103,7 +103,7 @@ GN_CASES = [
     (1, (1,), 8, 1), (2, (1, 1), 16, 16), (3, (5, 7), 24, 3), (2, (4, 4), 512, 32), (5, (13,), 72, 9),
     (2, (33, 31), 64, 32), (1, (64, 64), 64, 32), (2, (17, 19), 40, 8), (1, (9, 9), 2048, 1), (3, (3, 3), 88, 8),
     (2, (40, 41), 96, 2), (1, (1500,), 8, 8), (1, (6, 6), 4096, 2), (2, (50, 3), 136, 17), (1, (200, 100), 32, 4),
-    (4, (1000,), 56, 7),
+    (4, (1000,), 56, 7), (3, (9, 5), 4096, 1), (2, (70,), 8192, 2), (1, (4, 3), 3000, 1),
 ]
 
 
@@ -259,6 +259,19 @@ def test_linear(ops, case, dtype):
     lin_check(ops, x, w, None, res, dy, "lrelu", dtype, "lrelu")
 
 
+# The sizes at which the wider tiles are taken, with one to many stages of k, ends inside a tile, and rows that take copies
+# and single elements.
+@pytest.mark.parametrize("case", [(4096, 4096, 64), (4100, 4104, 136), (4096, 4099, 130), (4096, 4096, 328), (2056, 4104, 4100),
+                                  (1000, 1000, 2056), (2048, 2048, 72)], ids=lambda c: "x".join(map(str, c)))
+def test_linear_wide(ops, case):
+    M, N, K = case
+    g = torch.Generator(device="cuda").manual_seed(M + 7 * N + 31 * K)
+    x, w = rnd(g, M, K, dtype=BF), rnd(g, N, K, dtype=BF, scale=1 / math.sqrt(K))
+    bias, dy, res = rnd(g, N), rnd(g, M, N, dtype=BF), rnd(g, M, N, dtype=BF)
+    lin_check(ops, x, w, bias, res, dy, "gelu", F32, "gelu", pre_dtype=F32)
+    lin_check(ops, x, w, bias, None, dy, "none", BF, "none")
+
+
 @pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
 @pytest.mark.parametrize("size", [(70, 144, 136), (4, 272, 264), (300, 264, 520)])
 @pytest.mark.parametrize("off", [0, 1, 8])
@@ -387,7 +400,7 @@ def distill_check(ops, logits, tv, ti, w, T, scale, what, in_place=False):
 
 
 DIST_CASES = [(1, 1, 1), (3, 7, 7), (5, 100, 10), (64, 16, 3), (9, 1000, 64), (4, 1003, 130), (2, 8192, 128), (3, 32768, 64),
-              (2, 33333, 100), (2, 70001, 1024), (1, 131072, 128), (1, 140000, 33), (1, 300007, 5)]
+              (2, 33333, 100), (2, 70001, 1024), (9, 1500, 1024), (1, 131072, 128), (1, 140000, 33), (1, 300007, 5)]
 
 
 @pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])

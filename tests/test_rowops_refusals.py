@@ -133,6 +133,43 @@ def test_distill_pointers():
     assert "in place" in refused(f, C.byref(d), FAKE, FAKE, FAKE, None, FAKE, FAKE, FAKE, None)
 
 
+def test_sizes_beyond_a_launch():
+    """Row counters step past the end of the rows and a launch holds fewer than 2^32 threads: what would not fit is refused."""
+    from cvae_gan_amd._lib import lib, DistillDesc
+    d = C.byref(gn(B=1, HW=0x7fffffff))
+    assert "pixel rows" in refused(lib.cvg_gn_act_fwd, d, FAKE, None, FAKE, FAKE, FAKE, FAKE, FAKE, 1 << 62, None)
+    d = C.byref(gn(B=0x7fff0000, HW=1))
+    assert "too many" in refused(lib.cvg_gn_act_fwd, d, FAKE, None, FAKE, FAKE, FAKE, FAKE, FAKE, 1 << 62, None)
+    assert "too many" in refused(lib.cvg_gn_act_bwd, d, FAKE, FAKE, None, FAKE, None, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, 1 << 62, None)
+    for kw in (dict(M=64 << 12, N=64 << 10), dict(M=64 << 12, K=64 << 10, N=8), dict(M=1, N=64 << 11, K=64 << 11)):
+        d = C.byref(lin(**kw))
+        assert "too many" in refused(lib.cvg_linear_act_fwd, d, FAKE, FAKE, None, None, FAKE, None, FAKE, 1 << 62, None)
+        assert "too many" in refused(lib.cvg_linear_act_bwd, d, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, 1 << 62, None)
+    dd = DistillDesc()
+    dd.dtype, dd.R, dd.V, dd.top, dd.temperature = 1, 0x7fffffff, 1, 1, 1.0
+    assert "R 2147483647" in refused(lib.cvg_distill_topk, C.byref(dd), FAKE, FAKE, FAKE, None, FAKE, FAKE, FAKE, None)
+
+
+def test_outputs_over_inputs():
+    """An output may be the tensor the declaration names, at its pitch, and no other."""
+    from cvae_gan_amd._lib import lib
+    A, B_, D_, E = (FAKE + (i << 24) for i in range(4))
+    d = C.byref(gn(y_ld=128))
+    assert "in place" in refused(lib.cvg_gn_act_fwd, d, A, None, A, B_, B_, B_, E, 1 << 40, None)
+    assert "in place" in refused(lib.cvg_gn_act_fwd, d, A, D_, D_, B_, B_, B_, E, 1 << 40, None)
+    assert "in place" in refused(lib.cvg_gn_act_bwd, d, A, B_, None, A, None, E, E, E, E, E, E, 1 << 40, None)
+    assert "in place" in refused(lib.cvg_gn_act_bwd, d, A, B_, None, D_, A, E, E, E, E, E, E, 1 << 40, None)
+    for dx, dres in ((B_, None), (D_, None), (A, A), (A, B_), (A, D_)):
+        assert "another tensor" in refused(lib.cvg_gn_act_bwd, C.byref(gn()), A, B_, D_, dx, dres, E, E, E, E, E, E, 1 << 40, None)
+    d = C.byref(lin(M=64, y_ld=64))
+    fwd, bwd, F = lib.cvg_linear_act_fwd, lib.cvg_linear_act_bwd, FAKE + (9 << 24)
+    assert "in place" in refused(fwd, d, A, B_, None, D_, D_, None, E, 1 << 40, None)
+    for y, pre in ((A, None), (B_, None), (F, F), (F, A), (F, B_), (F, D_)):
+        assert "another tensor" in refused(fwd, d, A, B_, None, D_, y, pre, E, 1 << 40, None)
+    for dx, dw in ((A, None), (B_, None), (None, D_), (None, F)):
+        assert "another tensor" in refused(bwd, d, A, B_, D_, F, dx, dw, None, E, 1 << 40, None)
+
+
 def bad(call, needle):
     from cvae_gan_amd.ops import CvgError
     with pytest.raises(CvgError, match=needle):
