@@ -840,6 +840,7 @@ __device__ __forceinline__ void dz_body(const DzJob& a, int blk, float (*sm)[264
             float g[U][8], q[U][8];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
+                if (8 * u >= a.rows_blk) break;           // (few rows a block: no loads for rows that are not there)
                 const int64_t r = min(r0 + 8 * u, r1 - 1);
                 const T* gp = (const T*)a.dy + (size_t)r * a.dy_ld + c;
                 const P* qp = (const P*)a.pre + (size_t)r * a.pre_ld + c;
