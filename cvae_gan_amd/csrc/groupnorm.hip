@@ -7,6 +7,9 @@
 //   one tile per (sample, slab): the workgroup normalises its registers and writes y; x is read once.
 //   more than one: the tiles write (mean, M2) per group, a second kernel merges them (Chan's formula) and applies.
 // The backward pass is built the same way over per-channel sums of g and g * xhat, which also give dgamma / dbeta.
+// Bound by memory.  bf16, kernels alone: 256 x 32 x 32 x 128 with skip forward 35 us (200 MB); 256 x 64 x 64 x 64 forward
+// 75 us (3.6 TB/s) and backward 143 (2.8 TB/s: x and dy of one workgroup fill a CU's registers, so its loads, sums and
+// stores take turns; workgroups that walk over samples and load ahead were slower, 232 against 217 us for both).
 #include "rowops.h"
 
 namespace {
