@@ -650,3 +650,116 @@ def test_torch_operators(ops):
     ns.gn_act_bwd(b["dh"], t["x"], t["res"], b["dx"], b["dres"], 4, b["stats"], t["gamma"], t["beta"], b["dg"], b["dbt"], ops.ACT_SILU,
                   b["ws_gn"])
     assert all(torch.equal(p, q) for p, q in zip(ref, chain_outputs(b)))
+
+
+def pitched(rows, width, pitch, dtype):
+    """[rows, width] at a pitch that puts the last rows beyond 2^31 elements; the memory between the rows stays as it is."""
+    return torch.empty(rows * pitch, dtype=dtype, device="cuda").as_strided((rows, width), (pitch, 1))
+
+
+# 4000000 elements is a pitch that the tile kernel addresses directly, 6000000 one whose operands are copied and whose
+# outputs go element by element
+@pytest.mark.parametrize("pitch", [4000000, 6000000])
+def test_offsets_beyond_32_bits(ops, pitch):
+    """The same numbers at a pitch of megabytes and dense: the same results."""
+    g = torch.Generator(device="cuda").manual_seed(pitch)
+    M, N, K = 560, 72, 136
+
+    def far(t):
+        p = pitched(t.shape[0], t.shape[1], pitch, t.dtype)
+        p.copy_(t)
+        return p
+    x, w, dy, res = rnd(g, M, K, dtype=BF), rnd(g, N, K, dtype=BF), rnd(g, M, N, dtype=BF), rnd(g, M, N, dtype=BF)
+    got = []
+    for f in (lambda t: t.clone(), far):
+        xx, dd, rr = f(x), f(dy), f(res)
+        y, pre, dx = f(torch.zeros_like(res)), f(torch.zeros_like(res)), f(torch.zeros_like(x))
+        dw, db = torch.empty(N, K, device="cuda"), torch.empty(N, device="cuda")
+        ops.linear_act_fwd(xx, w, y, res=rr, pre=pre, act=ops.ACT_SILU)
+        ops.linear_act_bwd(dd, xx, w, pre=pre, dx=dx, dw=dw, dbias=db, act=ops.ACT_SILU)
+        one = f(torch.zeros_like(res))
+        ops.linear_act_fwd(xx[-20:], w, one[-20:], res=rr[-20:])
+        got.append([t.clone() for t in (y, pre, dx, dw, db, one[-20:])])
+        del xx, dd, rr, y, pre, dx, one
+    assert all(torch.equal(p, q) for p, q in zip(*got))
+    B, C, G = 2, 64, 8
+    x, dy = rnd(g, M, C, dtype=BF), rnd(g, M, C, dtype=BF)
+    gamma, beta = rnd(g, C, mean=1.0), rnd(g, C)
+    got = []
+    for f in (lambda t: t.clone(), far):
+        xx, dd, y, dx = [f(t).view(B, M // B, C) if f is not far else f(t).unflatten(0, (B, M // B)) for t in (x, dy, x, x)]
+        stats, dg, dbt = torch.empty(2, B, G, device="cuda"), torch.empty(C, device="cuda"), torch.empty(C, device="cuda")
+        ops.gn_act_fwd(xx, None, y, G, stats, gamma, beta, act=ops.ACT_SILU)
+        ops.gn_act_bwd(dd, xx, None, dx, None, G, stats, gamma, beta, dg, dbt, act=ops.ACT_SILU)
+        got.append([t.clone() for t in (y, dx, stats, dg, dbt)])
+        del xx, dd, y, dx
+    assert all(torch.equal(p, q) for p, q in zip(*got))
+    V = 3000
+    logits, tv = rnd(g, M, V, dtype=BF), rnd(g, M, 5)
+    ti = torch.randint(0, V, (M, 5), generator=g, device="cuda", dtype=torch.int32)
+    got = []
+    for f in (lambda t: t.clone(), far):
+        ll, dl = f(logits), f(torch.zeros_like(logits))
+        loss, rl = torch.empty((), device="cuda"), torch.empty(M, device="cuda")
+        ops.distill_topk(ll, tv, ti, loss, rl, dlogits=dl, temperature=2.0)
+        got.append([t.clone() for t in (loss, rl, dl)])
+        del ll, dl
+    assert all(torch.equal(p, q) for p, q in zip(*got))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("size", [(5, 48, 72), (130, 264, 264), (300, 77, 129)])
+def test_linear_gradients_one_at_a_time(ops, dtype, size):
+    """Every subset of the gradients is what the call for all of them gives."""
+    M, N, K = size
+    g = torch.Generator(device="cuda").manual_seed(M)
+    x, w, dy, pre = rnd(g, M, K, dtype=dtype), rnd(g, N, K, dtype=dtype), rnd(g, M, N, dtype=dtype), rnd(g, M, N)
+    for act in (ops.ACT_NONE, ops.ACT_GELU):
+        def run(which):
+            out = [torch.full(s, float("nan"), dtype=t, device="cuda") if i in which else None
+                   for i, (s, t) in enumerate((((M, K), dtype), ((N, K), F32), ((N,), F32)))]
+            ops.linear_act_bwd(dy, x, w, pre=pre, dx=out[0], dw=out[1], dbias=out[2], act=act)
+            return out
+        full = run((0, 1, 2))
+        for which in ((0,), (1,), (2,), (0, 1), (0, 2), (1, 2)):
+            for i, t in enumerate(run(which)):
+                assert (t is None) == (i not in which) and (t is None or torch.equal(t, full[i])), which
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+def test_vectors_at_any_element(ops, dtype):
+    """Parameter vectors, statistics and teacher entries that start on no 16-byte border; stats left out."""
+    g = torch.Generator(device="cuda").manual_seed(11)
+
+    def odd(t):
+        p = torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")[1:].view(t.shape)
+        return p.copy_(t)
+    for B, HW, C, G in ((3, 35, 40, 5), (1, 4096, 64, 8)):
+        x, dy, gamma, beta = rnd(g, B, HW, C, dtype=dtype), rnd(g, B, HW, C, dtype=dtype), rnd(g, C, mean=1.0), rnd(g, C)
+        got = []
+        for f in (torch.clone, odd):
+            y, dx, y2 = torch.empty_like(x), torch.empty_like(x), torch.empty_like(x)
+            st, dg, db = f(torch.zeros(2, B, G, device="cuda")), f(torch.zeros_like(gamma)), f(torch.zeros_like(gamma))
+            ops.gn_act_fwd(x, None, y, G, st, f(gamma), f(beta), act=ops.ACT_GELU)
+            ops.gn_act_fwd(x, None, y2, G, None, f(gamma), f(beta), act=ops.ACT_GELU)
+            ops.gn_act_bwd(dy, x, None, dx, None, G, st, f(gamma), f(beta), dg, db, act=ops.ACT_GELU)
+            assert torch.equal(y, y2)
+            got.append((y, dx, st, dg, db))
+        assert all(torch.equal(p, q) for p, q in zip(*got))
+    for M, N, K in ((7, 40, 32), (200, 136, 72)):
+        x, w, bias, dy = rnd(g, M, K, dtype=dtype), rnd(g, N, K, dtype=dtype), rnd(g, N), rnd(g, M, N, dtype=dtype)
+        got = []
+        for f in (torch.clone, odd):
+            y, db = torch.empty(M, N, dtype=dtype, device="cuda"), f(torch.zeros_like(bias))
+            ops.linear_act_fwd(x, w, y, bias=f(bias), act=ops.ACT_SILU)
+            ops.linear_act_bwd(dy, x, w, dbias=db)
+            got.append((y, db))
+        assert all(torch.equal(p, q) for p, q in zip(*got))
+    logits, tv, wt = rnd(g, 9, 1000, dtype=dtype), rnd(g, 9, 6), rnd(g, 9).abs()
+    ti = torch.randint(0, 1000, (9, 6), generator=g, device="cuda", dtype=torch.int32)
+    got = []
+    for f in (torch.clone, odd):
+        loss, rl, dl = f(torch.zeros(1, device="cuda")), f(torch.zeros(9, device="cuda")), torch.empty_like(logits)
+        ops.distill_topk(logits, f(tv), f(ti), loss, rl, dlogits=dl, row_weight=f(wt))
+        got.append((loss, rl, dl))
+    assert all(torch.equal(p, q) for p, q in zip(*got))
