@@ -293,9 +293,10 @@ template <typename T> struct Streams {
 //     of registers, a stage ahead of the LDS: fetching straight to LDS keeps the LDS busy for longer than writing 128 bytes
 //     a cycle does (8192 x 4096 x 4096 dw: staging alone takes 140 us, fragment reads alone 91, both together 221; the
 //     product with its 161 us of MFMAs 322).  dw 237 us (1160 TFLOP/s), dx 260, forward with f32 pre and residual 281.
-//   128 x 128 and 64 x 64: two workgroups share a CU and registers are short; direct-to-LDS loads.  Two LDS stages; the small
-//     tile, whose stages are over in a fraction of a load's latency, keeps four in flight.
-template <int BM> constexpr int ring() { return BM == 64 ? 4 : 2; }
+//   128 x 128 and 64 x 64: two or three workgroups share a CU and registers are short; direct-to-LDS loads.  Two LDS stages
+//     of 32 KB or three of 16: 512 x 4096 x 4096 by small tiles takes 31.9 us with two, 26.9 with three, 27.3 with four,
+//     550 x 8192 x 528 in f32 47.8, 48.7 and 51.5.
+template <int BM> constexpr int ring() { return BM == 64 ? 3 : 2; }
 template <typename T, int BM, int BN> struct TileLds {
     static constexpr int STAGES = ring<BM>() * (BM + BN) * 128, EPI = 4 * 32 * (BN / 2 * 4 + 16);
     static constexpr int BYTES = STAGES > EPI ? STAGES : EPI;
