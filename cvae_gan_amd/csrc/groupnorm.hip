@@ -34,9 +34,8 @@ struct Place {
     int b, tile, c0, chunk, ty, r0, r1, nv, nch, ngr, g0;
     bool live;
 };
-__device__ __forceinline__ Place gn_place(const GnArgs& a) {
+__device__ __forceinline__ Place gn_place(const GnArgs& a, uint32_t blk) {
     Place p;
-    uint32_t blk = blockIdx.x;
     uint32_t slab;
     if (a.tiles == 1) {
         // Workgroups go round-robin over the 8 dies: the slabs of one sample are given to one die, one after the other,
@@ -182,7 +181,7 @@ template <typename T, int ACT, int R, int MAXT, int WAVES>
 __global__ void __launch_bounds__(MAXT, WAVES) gn_fwd_tile(const GnArgs a) {
     extern __shared__ float sm[];
     __shared__ float sums[2][GN_MAX_GROUPS];
-    const Place p = gn_place(a);
+    const Place p = gn_place(a, blockIdx.x);
     const size_t row0 = (size_t)p.b * a.HW + p.r0;
     const int rows = p.r1 - p.r0, c = p.c0 + (p.live ? p.chunk * 8 : 0);
     float ga[8], be[8];                              // before the tile: what they wait for is short
@@ -267,7 +266,7 @@ __global__ void __launch_bounds__(MAXT, WAVES) gn_fwd_tile(const GnArgs a) {
 template <typename T, int ACT>
 __global__ void __launch_bounds__(512) gn_fwd_apply(const GnArgs a) {
     __shared__ float mu[GN_MAX_GROUPS], rs[GN_MAX_GROUPS];
-    const Place p = gn_place(a);
+    const Place p = gn_place(a, blockIdx.x);
     const int lane = threadIdx.x & 63, cg = a.cg.d;
     for (int g = threadIdx.x >> 6; g < p.ngr; g += blockDim.x >> 6) {
         const float* q = a.part + ((size_t)p.b * a.G + p.g0 + g) * a.tiles * 2;
@@ -348,7 +347,7 @@ template <typename T, int ACT, int R, bool RES, int MAXT, int WAVES>
 __global__ void __launch_bounds__(MAXT, WAVES) gn_bwd_tile(const GnArgs a) {
     extern __shared__ float sm[];
     __shared__ float sums[2][GN_MAX_GROUPS];
-    const Place p = gn_place(a);
+    const Place p = gn_place(a, blockIdx.x);
     const size_t row0 = (size_t)p.b * a.HW + p.r0;
     const int rows = p.r1 - p.r0, c = p.c0 + (p.live ? p.chunk * 8 : 0);
     int gi[8];
@@ -426,11 +425,46 @@ __global__ void __launch_bounds__(MAXT, WAVES) gn_bwd_tile(const GnArgs a) {
     }
 }
 
+// dgamma / dbeta from the partial rows [P][2][C] (P = samples * tiles): 16 columns by blockDim / 16 row lanes per workgroup
+struct ParamGrad {
+    const float* part;
+    float *dgamma, *dbeta;
+    int P, C, blocks;
+};
+__device__ __forceinline__ void param_grad(const ParamGrad& a, int blk, float (*sm)[17]) {
+    const int cl = threadIdx.x & 15, rl = threadIdx.x >> 4, lanes = blockDim.x >> 4, col = blk * 16 + cl;     // columns: dbeta, then dgamma
+    float s = 0.f;
+    if (col < 2 * a.C) {
+#pragma unroll 8
+        for (int i = rl; i < a.P; i += lanes) s += a.part[(size_t)i * 2 * a.C + col];
+    }
+    sm[rl][cl] = s;
+    __syncthreads();
+    if (threadIdx.x >= 64) return;
+    // one wave: 4 lanes per column, a quarter of the rows each
+    const int c = threadIdx.x & 15, q = threadIdx.x >> 4, per = lanes >> 2, cc = blk * 16 + c;
+    float t = 0.f;
+    for (int i = 0; i < per; ++i) t += sm[q * per + i][c];
+    t += __shfl_xor(t, 16, 64);
+    t += __shfl_xor(t, 32, 64);
+    if (q == 0 && cc < 2 * a.C) (cc < a.C ? a.dbeta : a.dgamma)[cc < a.C ? cc : cc - a.C] = t;
+}
+__global__ void __launch_bounds__(1024) gn_param_grad(const ParamGrad a) {
+    __shared__ float sm[64][17];
+    param_grad(a, blockIdx.x, sm);
+}
+
+// The first blocks take the parameters' gradients, which need the same partial sums: a launch less.
 template <typename T, int ACT, bool RES>
-__global__ void __launch_bounds__(512) gn_bwd_apply(const GnArgs a) {
+__global__ void __launch_bounds__(512) gn_bwd_apply(const GnArgs a, const ParamGrad pg) {
     extern __shared__ float sm[];            // [2][slab channels]
     __shared__ float sums[2][GN_MAX_GROUPS];
-    const Place p = gn_place(a);
+    __shared__ float pgm[32][17];
+    if ((int)blockIdx.x < pg.blocks) {
+        param_grad(pg, blockIdx.x, pgm);
+        return;
+    }
+    const Place p = gn_place(a, blockIdx.x - pg.blocks);
     const int width = a.nv * 8;
     const float* q = a.part + (size_t)p.b * a.tiles * 2 * a.C + p.c0;
     for (int t = threadIdx.x; t < 2 * width; t += blockDim.x) {
@@ -484,28 +518,6 @@ __global__ void __launch_bounds__(512) gn_bwd_apply(const GnArgs a) {
     }
 }
 
-// dgamma / dbeta from the partial rows [P][2][C] (P = samples * tiles): 16 columns by 64 row lanes per workgroup
-__global__ void __launch_bounds__(1024) gn_param_grad(const float* __restrict__ part, int P, int C, float* dgamma, float* dbeta) {
-    __shared__ float sm[64][17];
-    const int cl = threadIdx.x & 15, rl = threadIdx.x >> 4, col = blockIdx.x * 16 + cl;     // columns: dbeta, then dgamma
-    float s = 0.f;
-    if (col < 2 * C) {
-#pragma unroll 4
-        for (int i = rl; i < P; i += 64) s += part[(size_t)i * 2 * C + col];
-    }
-    sm[rl][cl] = s;
-    __syncthreads();
-    if (threadIdx.x >= 64) return;
-    // one wave: 4 lanes per column, 16 rows each
-    const int c = threadIdx.x & 15, q = threadIdx.x >> 4, cc = blockIdx.x * 16 + c;
-    float t = 0.f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) t += sm[q * 16 + i][c];
-    t += __shfl_xor(t, 16, 64);
-    t += __shfl_xor(t, 32, 64);
-    if (q == 0 && cc < 2 * C) (cc < C ? dbeta : dgamma)[cc < C ? cc : cc - C] = t;
-}
-
 // ---- planning ----------------------------------------------------------------------------------------------
 struct Plan {
     int nv, nslab, threads, R, tiles, rows_tile, rpp;
@@ -515,7 +527,7 @@ int gcd(int a, int b) { while (b) { const int t = a % b; a = b; b = t; } return 
 int check(const cvg_gn_desc* d, const char* who) {
     CVG_CHECK(d, "%s: null descriptor", who);
     CVG_CHECK(d->dtype == CVG_F32 || d->dtype == CVG_BF16, "%s: dtype %d", who, d->dtype);
-    CVG_CHECK(d->B >= 0 && d->HW >= 1 && d->C >= 8 && d->G >= 1, "%s: B %d, HW %d, C %d, G %d", who, d->B, d->HW, d->C, d->G);
+    CVG_CHECK(d->B >= 0 && d->HW >= 1 && d->C >= 8 && d->C <= 1 << 24 && d->G >= 1, "%s: B %d, HW %d, C %d, G %d", who, d->B, d->HW, d->C, d->G);
     CVG_CHECK(d->C % 8 == 0, "%s: C = %d is not a multiple of 8", who, d->C);
     CVG_CHECK(d->C % d->G == 0, "%s: %d groups do not divide %d channels", who, d->G, d->C);
     const int cg = d->C / d->G;
@@ -590,7 +602,9 @@ void fill(GnArgs& a, const cvg_gn_desc* d, const Plan& p) {
     a.cg = make_fastdiv(d->C / d->G); a.nvd = make_fastdiv(p.nv); a.tiled = make_fastdiv(p.tiles); a.slabd = make_fastdiv(p.nslab);
 }
 
-bool launchable(const cvg_gn_desc* d, const Plan& p) { return (int64_t)d->B * p.nslab * p.tiles * p.threads < (int64_t)1 << 32; }
+bool launchable(const cvg_gn_desc* d, const Plan& p) {
+    return ((int64_t)d->B * p.nslab * p.tiles + ceil_div(2 * d->C, 16)) * p.threads < (int64_t)1 << 32;
+}
 size_t ws_need(const cvg_gn_desc* d, const Plan& p, bool backward) {
     if (backward) return (size_t)d->B * p.tiles * 2 * d->C * 4;
     return p.tiles > 1 ? (size_t)d->B * d->G * p.tiles * 2 * 4 : 0;
@@ -609,7 +623,7 @@ void run_fwd(const GnArgs& a, const Plan& p, hipStream_t s) {
     if (p.tiles > 1) gn_fwd_apply<T, ACT><<<blocks, p.threads, 0, s>>>(a);
 }
 template <typename T, int ACT, bool RES>
-void run_bwd(GnArgs a, const Plan& p, hipStream_t s) {
+void run_bwd(GnArgs a, const Plan& p, ParamGrad pg, hipStream_t s) {
     const int blocks = a.B * p.nslab * p.tiles;
     const size_t lds = (size_t)a.ent * p.nv * 8 * 4 * 2;
     constexpr int RMAX = (sizeof(T) == 2 ? 16 : 8) / (RES ? 2 : 1);
@@ -619,19 +633,21 @@ void run_bwd(GnArgs a, const Plan& p, hipStream_t s) {
     else gn_bwd_tile<T, ACT, RMAX, RES, 512, 2><<<blocks, p.threads, lds, s>>>(a);
     if (p.tiles > 1) {
         a.ent = 1;
-        gn_bwd_apply<T, ACT, RES><<<blocks, p.threads, (size_t)2 * p.nv * 8 * 4, s>>>(a);
+        gn_bwd_apply<T, ACT, RES><<<blocks + pg.blocks, p.threads, (size_t)2 * p.nv * 8 * 4, s>>>(a, pg);
+    } else {
+        gn_param_grad<<<pg.blocks, 1024, 0, s>>>(pg);
     }
 }
 template <typename T, int ACT>
-void run_bwd(const GnArgs& a, const Plan& p, hipStream_t s) {
-    if (a.res) run_bwd<T, ACT, true>(a, p, s); else run_bwd<T, ACT, false>(a, p, s);
+void run_bwd(const GnArgs& a, const Plan& p, const ParamGrad& pg, hipStream_t s) {
+    if (a.res) run_bwd<T, ACT, true>(a, p, pg, s); else run_bwd<T, ACT, false>(a, p, pg, s);
 }
-#define GN_BY_ACT(run, T) \
+#define GN_BY_ACT(run, T, ...) \
     switch (a.act) { \
-        case CVG_ACT_LRELU: run<T, CVG_ACT_LRELU>(a, p, st); break; \
-        case CVG_ACT_SILU: run<T, CVG_ACT_SILU>(a, p, st); break; \
-        case CVG_ACT_GELU: run<T, CVG_ACT_GELU>(a, p, st); break; \
-        default: run<T, CVG_ACT_NONE>(a, p, st); \
+        case CVG_ACT_LRELU: run<T, CVG_ACT_LRELU>(a, p, __VA_ARGS__); break; \
+        case CVG_ACT_SILU: run<T, CVG_ACT_SILU>(a, p, __VA_ARGS__); break; \
+        case CVG_ACT_GELU: run<T, CVG_ACT_GELU>(a, p, __VA_ARGS__); break; \
+        default: run<T, CVG_ACT_NONE>(a, p, __VA_ARGS__); \
     }
 
 }  // namespace
@@ -665,7 +681,7 @@ int cvg_gn_act_fwd(const cvg_gn_desc* d, const void* x, const void* res, void* y
     fill(a, d, p);
     a.x = x; a.res = res; a.y = y; a.stats = stats; a.gamma = gamma; a.beta = beta; a.part = (float*)ws;
     hipStream_t st = (hipStream_t)s;
-    if (d->dtype == CVG_BF16) { GN_BY_ACT(run_fwd, bf16) } else { GN_BY_ACT(run_fwd, float) }
+    if (d->dtype == CVG_BF16) { GN_BY_ACT(run_fwd, bf16, st) } else { GN_BY_ACT(run_fwd, float, st) }
     CVG_LAUNCH_CHECK();
     return 0;
 }
@@ -691,11 +707,14 @@ int cvg_gn_act_bwd(const cvg_gn_desc* d, const void* dy, const void* x, const vo
     a.x = x; a.res = res; a.dy = dy; a.dx = dx; a.dres = dres; a.stats = (float*)stats; a.gamma = gamma; a.beta = beta;
     a.part = (float*)ws;
     hipStream_t st = (hipStream_t)s;
-    if (d->B > 0) {
-        if (d->dtype == CVG_BF16) { GN_BY_ACT(run_bwd, bf16) } else { GN_BY_ACT(run_bwd, float) }
-        CVG_LAUNCH_CHECK();
+    const ParamGrad pg{a.part, dgamma, dbeta, d->B * p.tiles, d->C, ceil_div(2 * d->C, 16)};
+    if (d->B == 0) {
+        gn_param_grad<<<pg.blocks, 1024, 0, st>>>(pg);          // (sums over nothing)
+    } else if (d->dtype == CVG_BF16) {
+        GN_BY_ACT(run_bwd, bf16, pg, st)
+    } else {
+        GN_BY_ACT(run_bwd, float, pg, st)
     }
-    gn_param_grad<<<ceil_div(2 * d->C, 16), 1024, 0, st>>>((const float*)ws, d->B * p.tiles, d->C, dgamma, dbeta);
     CVG_LAUNCH_CHECK();
     return 0;
 }

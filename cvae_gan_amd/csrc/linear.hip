@@ -939,10 +939,10 @@ int check(const cvg_linear_desc* d, const char* who) {
 // BM x BN tile takes `mfma` cycles of its matrix units, never less than the load latency a two-stage pipeline leaves
 // exposed; workgroups beyond one round queue up; K ranges add their f32 slabs (written and read once at ~2000 bytes per
 // cycle chip-wide) and a launch.  Forward bf16, us by 256 x 256 / 128 x 128 / 64 x 64 tiles:
-//   4096 x 4096 x 4096  116 / 131 / 204    2048 x 2048 x 2048  46 / 28 / 29    8192 x 1024 x 1024  35 / 23 / 31
-//   3000 x 3000 x 1000   39 /  41 /  45     512 x 4096 x 4096  45 / 35 / 27     550 x 8192 x  528  26 / 15 / 18
+//   4096 x 4096 x 4096  116 / 131 / 203    2048 x 2048 x 2048  46 / 28 / 29    8192 x 1024 x 1024  35 / 23 / 29
+//   3000 x 3000 x 1000   39 /  41 /  46     512 x 4096 x 4096  45 / 35 / 27     550 x 8192 x  528  26 / 15 / 16
 // f32, whose MFMAs take eight times as long and need no more bytes, always takes 64 x 64: 128 x 128 measured 1114 against
-// 1024 us at 4096 x 4096 x 4096, 217 against 160 at 3000 x 3000 x 1000.
+// 986 us at 4096 x 4096 x 4096, 217 against 148 at 3000 x 3000 x 1000.
 struct Tile { int cfg, splits, k_split; double t; };
 struct TileShape { int bm, bn, occ; double mfma; };
 const TileShape TILES[2][3] = {{{0, 0, 0, 0}, {0, 0, 0, 0}, {64, 64, 2, 1024 / .7}},

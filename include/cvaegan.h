@@ -463,7 +463,7 @@ enum { CVG_ACT_NONE = 0, CVG_ACT_LRELU = 1 /* slope 0.2 */, CVG_ACT_SILU = 2, CV
  * variance) over the HW pixels and C / G channels of one sample and group.
  * Tensors are [B * HW] pixel rows of C channels at the pitches of the descriptor (elements, 0 = C).  C is a multiple
  * of 8, G divides C, the least common multiple of 8 and C / G is at most 4096; pointers are 16-byte aligned and
- * pitches multiples of 16 bytes.  B may be 0; B * HW is at most 0x7fff0000.
+ * pitches multiples of 16 bytes.  B may be 0; B * HW is at most 0x7fff0000, C at most 0x1000000.
  * stats f32 [2][B][G] = mean, rstd: written by the forward call, read by the backward call.
  * y may be x or res itself, at the same pitch; other overlaps of an output with an input are not supported.  */
 typedef struct cvg_gn_desc {

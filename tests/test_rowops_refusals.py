@@ -138,6 +138,8 @@ def test_sizes_beyond_a_launch():
     from cvae_gan_amd._lib import lib, DistillDesc
     d = C.byref(gn(B=1, HW=0x7fffffff))
     assert "pixel rows" in refused(lib.cvg_gn_act_fwd, d, FAKE, None, FAKE, FAKE, FAKE, FAKE, FAKE, 1 << 62, None)
+    d = C.byref(gn(B=1, HW=1, C=1 << 30, G=1 << 27))
+    assert "C 1073741824" in refused(lib.cvg_gn_act_fwd, d, FAKE, None, FAKE, FAKE, FAKE, FAKE, FAKE, 1 << 62, None)
     d = C.byref(gn(B=0x7fff0000, HW=1))
     assert "too many" in refused(lib.cvg_gn_act_fwd, d, FAKE, None, FAKE, FAKE, FAKE, FAKE, FAKE, 1 << 62, None)
     assert "too many" in refused(lib.cvg_gn_act_bwd, d, FAKE, FAKE, None, FAKE, None, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, 1 << 62, None)
