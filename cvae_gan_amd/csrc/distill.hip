@@ -18,6 +18,15 @@ namespace {
 
 constexpr int MAX_TOP = 1024;
 
+// e^(d / T) for d <= 0, as 2^(d k): k = log2(e) / T.  For f32 logits in two parts, hi rounded towards zero and lo > 0 (so
+// -inf stays -inf): one part alone puts the same relative error times d k into every exponential, and none of it averages
+// out (256 x 100, T = 2: 4.9e-7 of the gradient, against 2.3e-7).  bf16 logits carry 2^-9 of their own; there the
+// multiply-add more per element would cost 3 % of the time.
+struct Scale { float hi, lo; };
+template <typename T> __device__ __forceinline__ float exp_t(const Scale& k, float d) {
+    return __builtin_amdgcn_exp2f(sizeof(T) == 4 ? fmaf(d, k.lo, d * k.hi) : d * k.hi);
+}
+
 struct DistillArgs {
     const void* logits;
     const float* top_val;
@@ -27,6 +36,7 @@ struct DistillArgs {
     void* dlogits;
     int R, V, top;
     size_t ld, dld, tld;
+    Scale k;
     float inv_t, temp, scale;
 };
 
@@ -43,26 +53,23 @@ template <int TPR> __device__ __forceinline__ float row_sum(float v, float* sh) 
     return s;
 }
 
-#define LOG2E 1.4426950408889634f
-__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
-
-// Running (maximum, sum of 2^(k (v - maximum))).  The maximum is subtracted before k is multiplied in: k times the lowest
+// Running (maximum, sum of e^((v - maximum) / T)).  The maximum is subtracted before k is multiplied in: k times the lowest
 // values of a type overflows, and a row that is masked throughout is uniform.  It starts at the lowest finite value, so
 // that a row may begin with -inf; a NaN or +inf reaches the sum.
-struct Running {
+template <typename T> struct Running {
     float m, s;
-    __device__ __forceinline__ void add(const float (&v)[8], float k) {
+    __device__ __forceinline__ void add(const float (&v)[8], const Scale& k) {
         const float before = m;
 #pragma unroll
         for (int j = 0; j < 8; ++j) m = v[j] > m ? v[j] : m;
         float t = 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) t += exp2_((v[j] - m) * k);
-        s = fmaf(s, exp2_((before - m) * k), t);
+        for (int j = 0; j < 8; ++j) t += exp_t<T>(k, v[j] - m);
+        s = fmaf(s, exp_t<T>(k, before - m), t);
     }
-    __device__ __forceinline__ void join(float m2, float s2, float k) {
+    __device__ __forceinline__ void join(float m2, float s2, const Scale& k) {
         const float n = fmaxf(m, m2);
-        s = s * exp2_((m - n) * k) + s2 * exp2_((m2 - n) * k);
+        s = s * exp_t<T>(k, m - n) + s2 * exp_t<T>(k, m2 - n);
         m = n;
     }
 };
@@ -123,7 +130,7 @@ __global__ void __launch_bounds__(TPR == 64 ? 256 : TPR, 4) distill_row(const Di
     float* tp = tv + 2 * a.top;
     int32_t* next = (int32_t*)(tv + 3 * a.top);
     int32_t* head = heads[sub];
-    const float k = a.inv_t * LOG2E;
+    const Scale k = a.k;
     const int stride = gridDim.x * ROWS;
     constexpr uint32_t VB = 8 * sizeof(T);               // bytes of a vector
 
@@ -150,13 +157,13 @@ __global__ void __launch_bounds__(TPR == 64 ? 256 : TPR, 4) distill_row(const Di
         T* out = a.dlogits ? (T*)a.dlogits + (size_t)r * a.dld : nullptr;
         const bool whole = EVEN || (out && ((((uintptr_t)out) ^ (uintptr_t)row) & 15) == 0);
         // ---- the teacher: entries into LDS, their maximum and sum, chains by vector
-        float v0 = ev * a.inv_t;
+        float v0 = ev;
         int c0 = ei;
         if (c0 < 0 || c0 >= a.V || v0 == -INFINITY) { c0 = -1; v0 = -INFINITY; }
         float s0 = to_f32(row[max(c0, 0)]);               // the student's logit at this thread's first class
         if (tid < a.top) { tv[tid] = v0; ti[tid] = c0; }
         for (int j = tid + TPR; j < a.top; j += TPR) {
-            const float v = a.top_val[(size_t)r * a.tld + j] * a.inv_t;
+            const float v = a.top_val[(size_t)r * a.tld + j];
             const int c = a.top_idx[(size_t)r * a.tld + j];
             const bool in = c >= 0 && c < a.V && v != -INFINITY;
             tv[j] = in ? v : -INFINITY;
@@ -168,14 +175,15 @@ __global__ void __launch_bounds__(TPR == 64 ? 256 : TPR, 4) distill_row(const Di
         for (int j = lane; j < a.top; j += 64) tmax = fmaxf(tmax, tv[j]);
         tmax = wave_max(tmax);
         for (int j = lane; j < a.top; j += 64)
-            if (ti[j] >= 0) ps += expf(tv[j] - tmax);
+            if (ti[j] >= 0) ps += expf((tv[j] - tmax) * a.inv_t);
         ps = wave_sum(ps);                                // 0: no entry at all (the largest adds 1, a NaN stays)
         const bool dead = w == 0.f || ps == 0.f;
-        const float logp0 = logf(ps) + tmax;
+        const float inv_ps = 1.f / ps;
+        auto share = [&](int j) { return expf((tv[j] - tmax) * a.inv_t) * inv_ps; };      // p of entry j
         if (!dead)
             for (int j = tid; j < a.top; j += TPR) {
                 const int c = ti[j];
-                if (c < 0 || expf(tv[j] - logp0) == 0.f) { next[j] = -2; continue; }      // (absent, or nothing to add)
+                if (c < 0 || share(j) == 0.f) { next[j] = -2; continue; }      // (absent, or nothing to add)
                 next[j] = atomicExch(&head[((c + off) >> 3) & (HASH - 1)], j);
             }
         row_barrier<TPR>();
@@ -192,14 +200,14 @@ __global__ void __launch_bounds__(TPR == 64 ? 256 : TPR, 4) distill_row(const Di
                             if (q > last && q < e && ti[q] == c) e = q;
                         if (last < 0 && e != j) break;    // (not the first)
                         if (e == MAX_TOP) break;
-                        p += expf(tv[e] - logp0);
+                        p += share(e);
                         last = e;
                     }
                 }
                 tp[j] = p;
             }
         // ---- maximum and sum
-        Running run{-3.402823466e38f, 0.f};
+        Running<T> run{-3.402823466e38f, 0.f};
         if constexpr (R > 0) {
 #pragma unroll
             for (int u = 0; u < R; ++u) {
@@ -229,15 +237,15 @@ __global__ void __launch_bounds__(TPR == 64 ? 256 : TPR, 4) distill_row(const Di
             for (int i = 1; i < TPR / 64; ++i) run.join(sh[i], sh[16 + i], k);
         }
         const float m = run.m, inv_z = 1.f / run.s, c = a.scale * w * a.temp, cz = c * inv_z;
-        // ---- the loss: T^2 p (log p - log q) as T p (T log p - ((s - maximum) - T log z)), which does not divide a masked
-        // logit by a temperature below one
+        // ---- the loss: T^2 p (log p - log q) as T p ((t - its maximum) - T log(its sum) - ((s - maximum) - T log z)), which
+        // does not divide a masked logit by a temperature below one
         float l = 0.f;
         if (!dead) {
-            const float tz = a.temp * logf(run.s), wt = w * a.temp;
+            const float tz = a.temp * logf(run.s), tp0 = a.temp * logf(ps), wt = w * a.temp;
             for (int j = tid; j < a.top; j += TPR) {
                 if (next[j] == -2) continue;
-                const float lp = tv[j] - logp0, v = j == tid ? s0 : to_f32(row[ti[j]]);
-                l += wt * expf(lp) * (a.temp * lp - ((v - m) - tz));
+                const float v = j == tid ? s0 : to_f32(row[ti[j]]);
+                l += wt * share(j) * (((tv[j] - tmax) - tp0) - ((v - m) - tz));
             }
         }
         // ---- the gradient; the next row moves in
@@ -255,7 +263,7 @@ __global__ void __launch_bounds__(TPR == 64 ? 256 : TPR, 4) distill_row(const Di
         }
         auto gradient = [&](float (&v)[8], int i) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = cz * exp2_((v[j] - m) * k);
+            for (int j = 0; j < 8; ++j) v[j] = cz * exp_t<T>(k, v[j] - m);
             for (int q = head[i & (HASH - 1)]; q >= 0; q = next[q]) {
                 const int at = ti[q] + off - 8 * i;
                 const float p = c * tp[q];
@@ -377,7 +385,7 @@ extern "C" int cvg_distill_topk(const cvg_distill_desc* d, const void* logits, c
     CVG_CHECK(d->R >= 0 && d->V >= 1, "distill_topk: R %d, V %d", d->R, d->V);
     CVG_CHECK(d->R <= 0x7fff0000 && d->V <= 0x7ffffff0, "distill_topk: R %d, V %d", d->R, d->V);   // (row loops step past the end)
     CVG_CHECK(d->top >= 1 && d->top <= MAX_TOP, "distill_topk: %d teacher entries (1..%d)", d->top, MAX_TOP);
-    CVG_CHECK(d->temperature > 0.f && d->temperature < INFINITY, "distill_topk: temperature %g", (double)d->temperature);
+    CVG_CHECK(d->temperature >= 1e-37f && d->temperature < INFINITY, "distill_topk: temperature %g", (double)d->temperature);
     CVG_CHECK((d->logits_ld == 0 || d->logits_ld >= d->V) && (d->dlogits_ld == 0 || d->dlogits_ld >= d->V) &&
               (d->top_ld == 0 || d->top_ld >= d->top), "distill_topk: pitches %d, %d, %d", d->logits_ld, d->dlogits_ld, d->top_ld);
     CVG_CHECK(loss, "distill_topk: null loss");
@@ -392,6 +400,11 @@ extern "C" int cvg_distill_topk(const cvg_distill_desc* d, const void* logits, c
     a.dld = d->dlogits_ld ? d->dlogits_ld : d->V;
     a.tld = d->top_ld ? d->top_ld : d->top;
     a.temp = d->temperature; a.inv_t = 1.f / d->temperature; a.scale = d->grad_scale;
+    const double k = 1.4426950408889634 / (double)d->temperature;
+    a.k.hi = (float)k;
+    if (d->dtype == CVG_F32 && (double)a.k.hi > k) a.k.hi = nextafterf(a.k.hi, 0.f);
+    a.k.lo = (float)(k - (double)a.k.hi);
+    if (!(a.k.lo > 0.f)) a.k.lo = 1e-30f;
     CVG_CHECK(dlogits != logits || a.ld == a.dld, "distill_topk: in place with different pitches");
     hipStream_t st = (hipStream_t)s;
     if (d->R > 0) {

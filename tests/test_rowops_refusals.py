@@ -108,7 +108,7 @@ def test_linear_pointers_and_workspaces():
 @pytest.mark.parametrize("kw, needle", [
     (dict(dtype=5), "dtype"), (dict(V=0), "V 0"), (dict(R=-2), "R -2"), (dict(top=0), "teacher entries"), (dict(top=1025), "teacher entries"),
     (dict(temperature=0.0), "temperature"), (dict(temperature=-1.0), "temperature"), (dict(temperature=float("nan")), "temperature"),
-    (dict(temperature=float("inf")), "temperature"), (dict(logits_ld=99), "pitches"), (dict(dlogits_ld=1), "pitches"),
+    (dict(temperature=float("inf")), "temperature"), (dict(temperature=1e-39), "temperature"), (dict(logits_ld=99), "pitches"), (dict(dlogits_ld=1), "pitches"),
     (dict(top_ld=3), "pitches"),
 ])
 def test_distill_descriptors(kw, needle):
