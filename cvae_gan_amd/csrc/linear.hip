@@ -626,29 +626,34 @@ __global__ void __launch_bounds__(256) gemm_tile(const GemmArgs a) {
     tile_body<T, BM, BN, ACOL, BCOL>(a, blockIdx.x, blockIdx.y, lds);
 }
 
-// ---- few rows: M <= 16 MT ------------------------------------------------------------------------------------
+// ---- few rows: M <= 16 ---------------------------------------------------------------------------------------
 // The weights are all there is to read.  A workgroup takes 16 of their rows; its eight waves take turns along k, 64 values
 // (a whole cache line of a bf16 row) at a time, straight from memory into 16 x 16 MFMA fragments: lane (r, q) holds k
 // values 16 q .. 16 q + 15 of the unit, of weight row r and of x row r alike, so any order of k inside the unit is right as
-// long as both operands share it.  x rows beyond M are zero.  The waves' sums meet in LDS in wave order; no second launch.
-// One token through 4096 x 4096 bf16: 34 MB in 8.0 us (4.2 TB/s).
+// long as both operands share it.  Units come in two sets, one on its way while the other is multiplied; what lies behind
+// K, and x rows beyond M, read as zeros.  The waves' sums meet in LDS in wave order; no second launch, no workspace.
+// One token through 4096 x 4096 bf16: 34 MB in @BF@ us; f32: 67 MB in @F32@.  Every workgroup reads all of x, from 17 rows
+// on more than its weights: @ROWS@
 template <typename T> struct Unit;                                // 16 consecutive k of one row
 template <> struct Unit<bf16> { u32x4 a[2]; };
 template <> struct Unit<float> { u32x4 a[4]; };
+// `at`: byte offset of the row from base, or -1 for a row of zeros
 template <typename T, bool ALIGNED>
-__device__ __forceinline__ void unit_load(Unit<T>& u, const T* row, int k, int K, bool live) {
+__device__ __forceinline__ void unit_load(Unit<T>& u, const char* base, int at, const T* row, int k, int K) {
     constexpr int PER = 16 / sizeof(T), NV = 16 / PER;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int kk = k + i * PER;
-        u.a[i] = u32x4{0, 0, 0, 0};
-        if constexpr (ALIGNED) {
-            if (live && kk < K) u.a[i] = *(const u32x4*)(row + kk);       // (K is a multiple of 16 bytes)
-        } else if (live) {
-            T t[PER];
+        if constexpr (ALIGNED) {                                  // (K is a multiple of 16 bytes)
+            u.a[i] = buf_load(base, 0x7fffffff, at >= 0 && kk < K ? at + kk * (int)sizeof(T) : -1);
+        } else {
+            u.a[i] = u32x4{0, 0, 0, 0};
+            if (at >= 0) {
+                T t[PER];
 #pragma unroll
-            for (int j = 0; j < PER; ++j) t[j] = kk + j < K ? row[kk + j] : from_f32<T>(0.f);
-            u.a[i] = __builtin_bit_cast(u32x4, *(T (*)[PER])t);
+                for (int j = 0; j < PER; ++j) t[j] = kk + j < K ? row[kk + j] : from_f32<T>(0.f);
+                u.a[i] = __builtin_bit_cast(u32x4, *(T (*)[PER])t);
+            }
         }
     }
 }
@@ -664,43 +669,63 @@ __device__ __forceinline__ void unit_mma(f32x4& acc, const Unit<float>& w, const
         for (int j = 0; j < 4; ++j)
             acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(w.a[i][j]), __uint_as_float(x.a[i][j]), acc, 0, 0, 0);
 }
-template <typename T, int MT, bool ALIGNED>
+template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(512) few_rows(const GemmArgs a) {
-    constexpr int U = (sizeof(T) == 2 && ALIGNED ? 8 : 4) / MT;   // units in flight per wave
-    __shared__ float red[8][MT][16][17];
+    constexpr int U = ALIGNED && sizeof(T) == 2 ? 4 : 2;          // units of a set
+    __shared__ float red[8][16][17];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4, n0 = blockIdx.x * 16;
-    const T* w = (const T*)a.B + (size_t)min(n0 + r, a.N - 1) * a.ldb;
-    f32x4 acc[MT];
+    const char* wb = (const char*)((const T*)a.B + (size_t)n0 * a.ldb);
+    const int wr = min(r, a.N - 1 - n0);
+    const T *w = (const T*)wb + wr * a.ldb, *x = (const T*)a.A + min(r, a.M - 1) * a.lda;
+    // (pitches of the aligned form are at most MAX_PITCH)
+    const int w_at = ALIGNED ? wr * (int)(a.ldb * sizeof(T)) : 0, x_at = r >= a.M ? -1 : ALIGNED ? r * (int)(a.lda * sizeof(T)) : 0;
+    f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+    Unit<T> uw[2][U], ux[2][U];
+    auto load = [&](int set, int k0) {
 #pragma unroll
-    for (int t = 0; t < MT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int k0 = wave * 64; k0 < a.K; k0 += U * 512) {
-        Unit<T> uw[U], ux[U][MT];
+        for (int u = 0; u < U; ++u) unit_load<T, ALIGNED>(uw[set][u], wb, w_at, w, k0 + u * 512 + q * 16, a.K);
 #pragma unroll
-        for (int u = 0; u < U; ++u) unit_load<T, ALIGNED>(uw[u], w, k0 + u * 512 + q * 16, a.K, true);
+        for (int u = 0; u < U; ++u) unit_load<T, ALIGNED>(ux[set][u], (const char*)a.A, x_at, x, k0 + u * 512 + q * 16, a.K);
+    };
+    auto multiply = [&](int set) {
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+        for (int u = 0; u < U; ++u) unit_mma(acc, uw[set][u], ux[set][u]);
+    };
+    const int k_wave = __builtin_amdgcn_readfirstlane(wave) * 64;
+    if (a.K <= 2 * U * 512) {                                     // all of it at once, and nothing that is not there
 #pragma unroll
-            for (int t = 0; t < MT; ++t)
-                unit_load<T, ALIGNED>(ux[u][t], (const T*)a.A + (size_t)min(t * 16 + r, a.M - 1) * a.lda, k0 + u * 512 + q * 16, a.K, t * 16 + r < a.M);
+        for (int u = 0; u < 2 * U; ++u)
+            if (k_wave + u * 512 < a.K) unit_load<T, ALIGNED>(uw[u / U][u % U], wb, w_at, w, k_wave + u * 512 + q * 16, a.K);
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+        for (int u = 0; u < 2 * U; ++u)
+            if (k_wave + u * 512 < a.K) unit_load<T, ALIGNED>(ux[u / U][u % U], (const char*)a.A, x_at, x, k_wave + u * 512 + q * 16, a.K);
 #pragma unroll
-            for (int t = 0; t < MT; ++t) unit_mma(acc[t], uw[u], ux[u][t]);
+        for (int u = 0; u < 2 * U; ++u)
+            if (k_wave + u * 512 < a.K) unit_mma(acc, uw[u / U][u % U], ux[u / U][u % U]);
+    } else {
+        int k0 = k_wave;
+        load(0, k0);
+        load(1, k0 + U * 512);
+        for (; k0 + 2 * U * 512 < a.K; k0 += 2 * U * 512) {
+            multiply(0);
+            load(0, k0 + 2 * U * 512);
+            multiply(1);
+            load(1, k0 + 3 * U * 512);
+        }
+        multiply(0);
+        multiply(1);
     }
     // lane (r, q): x row r, weight rows 4 q .. 4 q + 3
 #pragma unroll
-    for (int t = 0; t < MT; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) red[wave][t][r][4 * q + i] = acc[t][i];
+    for (int i = 0; i < 4; ++i) red[wave][r][4 * q + i] = acc[i];
     __syncthreads();
-    for (int i = threadIdx.x; i < MT * 256; i += 512) {
-        const int n = i & 15, m = i >> 4;
-        if (m >= a.M || n0 + n >= a.N) continue;
-        float v = 0.f;
+    if (threadIdx.x >= 256) return;
+    const int n = threadIdx.x & 15, m = threadIdx.x >> 4;
+    if (m >= a.M || n0 + n >= a.N) return;
+    float v = 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v += red[j][m >> 4][m & 15][n];
-        emit<T>(a.e, m, n0 + n, v);
-    }
+    for (int j = 0; j < 8; ++j) v += red[j][m][n];
+    emit<T>(a.e, m, n0 + n, v);
 }
 
 // column sums of [P][N] partial rows: 32 columns by `blockDim / 32` row lanes
@@ -915,7 +940,7 @@ size_t round_up(size_t v, size_t to) { return (v + to - 1) / to * to; }
 size_t max_sz(size_t a, size_t b) { return a > b ? a : b; }
 
 // the tile kernel's lane offsets span 256 rows in 31 bits
-constexpr int FEW_ROWS = 32;
+constexpr int FEW_ROWS = 16;
 constexpr int MAX_WIDTH = 2000000;
 constexpr size_t MAX_PITCH = ((size_t)1 << 31) / 256 - 64;       // bytes
 
@@ -1103,11 +1128,7 @@ int forward(const cvg_linear_desc* d, const void* x, const void* w, const float*
         a.A = X.p; a.B = W.p; a.lda = X.ld; a.ldb = W.ld; a.M = d->M; a.N = d->N; a.K = d->K; a.e = e;
         const bool al = fits(X, sizeof(T)) && fits(W, sizeof(T));
         const int blocks = ceil_div(d->N, 16);
-        if (d->M <= 16) {
-            if (al) few_rows<T, 1, true><<<blocks, 512, 0, s>>>(a); else few_rows<T, 1, false><<<blocks, 512, 0, s>>>(a);
-        } else {
-            if (al) few_rows<T, 2, true><<<blocks, 512, 0, s>>>(a); else few_rows<T, 2, false><<<blocks, 512, 0, s>>>(a);
-        }
+        if (al) few_rows<T, true><<<blocks, 512, 0, s>>>(a); else few_rows<T, false><<<blocks, 512, 0, s>>>(a);
         CVG_LAUNCH_CHECK();
         return 0;
     }
