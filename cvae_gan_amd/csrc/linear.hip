@@ -632,8 +632,7 @@ __global__ void __launch_bounds__(256) gemm_tile(const GemmArgs a) {
 // values 16 q .. 16 q + 15 of the unit, of weight row r and of x row r alike, so any order of k inside the unit is right as
 // long as both operands share it.  Units come in two sets, one on its way while the other is multiplied; what lies behind
 // K, and x rows beyond M, read as zeros.  The waves' sums meet in LDS in wave order; no second launch, no workspace.
-// One token through 4096 x 4096 bf16: 34 MB in @BF@ us; f32: 67 MB in @F32@.  Every workgroup reads all of x, from 17 rows
-// on more than its weights: @ROWS@
+// Bound by memory: one token through 4096 x 4096 bf16, 34 MB, takes 8.0 us (4.2 TB/s), through 16384 x 4096 28 (4.8 TB/s).
 template <typename T> struct Unit;                                // 16 consecutive k of one row
 template <> struct Unit<bf16> { u32x4 a[2]; };
 template <> struct Unit<float> { u32x4 a[4]; };
@@ -940,7 +939,6 @@ size_t round_up(size_t v, size_t to) { return (v + to - 1) / to * to; }
 size_t max_sz(size_t a, size_t b) { return a > b ? a : b; }
 
 // the tile kernel's lane offsets span 256 rows in 31 bits
-constexpr int FEW_ROWS = 16;
 constexpr int MAX_WIDTH = 2000000;
 constexpr size_t MAX_PITCH = ((size_t)1 << 31) / 256 - 64;       // bytes
 
@@ -1091,10 +1089,17 @@ int multiply(GemmArgs& a, bool acol, bool bcol, const Tile& t, hipStream_t s) {
     return sum_slabs<T>(slab_job<T>(a, t), SlabJob{}, s);
 }
 
+// Few rows: every workgroup of few_rows reads all of x, from 17 rows on more than its weights (32 rows of 4096 x 4096 bf16:
+// 15.8 us, 14.0 by tiles).  Long rows of few weights leave most CUs without one of its workgroups, and a product split
+// along k is faster in spite of its second launch (16 rows, us by few_rows / by tiles, bf16):
+//   1024 x 8192 16.2 / 10.1    2048 x 8192 18.0 / 13.5    1024 x 4096 9.2 / 9.0    1024 x 2048 5.7 / 8.8    2048 x 2048 6.0 / 8.7
+// and f32: 1024 x 4096 16.6 / 12.9, 1024 x 2048 9.9 / 10.5.
+bool takes_few_rows(const cvg_linear_desc* d) { return d->M <= 16 && (d->K * es_of(d->dtype) <= 8192 || d->N > 2048); }
+
 // Workspaces: dz, partial column sums, padded copies, slabs.  The sizes do not depend on pitches or alignment, so one
 // workspace serves every call of the same shape.
 size_t fwd_ws(const cvg_linear_desc* d) {
-    if (d->M <= FEW_ROWS) return 0;
+    if (d->M == 0 || takes_few_rows(d)) return 0;
     const size_t es = es_of(d->dtype);
     return padded_bytes(d->M, d->K, es) + padded_bytes(d->N, d->K, es) + slab_of(choose(d->dtype, d->M, d->N, d->K), d->M, d->N);
 }
@@ -1123,7 +1128,7 @@ int forward(const cvg_linear_desc* d, const void* x, const void* w, const float*
     e.bias = bias; e.res = res; e.pre = pre; e.out = y; e.act = d->act;
     e.out_f32 = 0; e.pre_f32 = sizeof(T) == 2 && d->pre_dtype == CVG_F32;
     e.res_ld = ld_of(d->res_ld, d->N); e.pre_ld = ld_of(d->pre_ld, d->N); e.out_ld = ld_of(d->y_ld, d->N);
-    if (d->M <= FEW_ROWS) {
+    if (takes_few_rows(d)) {
         GemmArgs a{};
         a.A = X.p; a.B = W.p; a.lda = X.ld; a.ldb = W.ld; a.M = d->M; a.N = d->N; a.K = d->K; a.e = e;
         const bool al = fits(X, sizeof(T)) && fits(W, sizeof(T));

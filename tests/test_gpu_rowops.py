@@ -212,7 +212,7 @@ LIN_CASES = [
     # M, N, K
     (1, 1, 1), (1, 64, 64), (1, 1000, 515), (2, 24, 8), (3, 136, 72), (16, 256, 512), (17, 100, 33), (33, 48, 200),
     (64, 512, 128), (100, 77, 129), (130, 264, 264), (256, 128, 1096), (300, 520, 96), (515, 9, 17), (777, 303, 115), (513, 512, 320),
-    (1, 4096, 1032), (5, 2056, 24), (48, 640, 1024), (2048, 40, 8), (1030, 776, 200),
+    (1, 4096, 1032), (3, 264, 8200), (16, 40, 4104), (1, 2056, 4104), (5, 2056, 24), (48, 640, 1024), (2048, 40, 8), (1030, 776, 200),
 ]
 
 
