@@ -745,20 +745,24 @@ __device__ __forceinline__ void sum_rows_body(const float* __restrict__ part, in
 struct SumArgs { const float* part; float* out; int P, N; };
 
 // Both gradients of a layer in one launch: neither waits for the other, small ones do not fill the chip alone, and a
-// launch costs as much as they do.  The blocks behind the two products finish the bias gradient.
+// launch costs as much as they do.  The first blocks finish the bias gradient; the product with the longer range of k goes
+// ahead of the other, so that what starts last is over soonest.
 template <typename T, int BM, int BN>
-__global__ void __launch_bounds__(256) gemm_pair(const GemmArgs dx, const GemmArgs dw, int blocks_dx, int blocks_dw, const SumArgs db) {
+__global__ void __launch_bounds__(256) gemm_pair(const GemmArgs dx, const GemmArgs dw, int blocks_dx, int blocks_dw, int blocks_db, const SumArgs db) {
     __shared__ __attribute__((aligned(1024))) char lds[TileLds<T, BM, BN>::BYTES];
-    int blk = blockIdx.x;
-    if (blk < blocks_dx) {
-        const int nt = dx.tiles_m * dx.tiles_n, slice = blk / nt;
-        tile_body<T, BM, BN, false, true>(dx, blk - slice * nt, slice, lds);
-    } else if (blk < blocks_dx + blocks_dw) {
-        blk -= blocks_dx;
+    int blk = blockIdx.x - blocks_db;
+    if (blk < 0) {
+        sum_rows_body(db.part, db.P, db.N, db.out, blockIdx.x, (float (*)[32])lds);
+        return;
+    }
+    const bool dw_first = dw.k_split > dx.k_split, is_dw = dw_first ? blk < blocks_dw : blk >= blocks_dx;
+    if (is_dw != dw_first) blk -= dw_first ? blocks_dw : blocks_dx;
+    if (is_dw) {
         const int nt = dw.tiles_m * dw.tiles_n, slice = blk / nt;
         tile_body<T, BM, BN, true, true>(dw, blk - slice * nt, slice, lds);
     } else {
-        sum_rows_body(db.part, db.P, db.N, db.out, blk - blocks_dx - blocks_dw, (float (*)[32])lds);
+        const int nt = dx.tiles_m * dx.tiles_n, slice = blk / nt;
+        tile_body<T, BM, BN, false, true>(dx, blk - slice * nt, slice, lds);
     }
 }
 __global__ void __launch_bounds__(256) sum_rows(const SumArgs a) {
@@ -1190,9 +1194,9 @@ int backward(const cvg_linear_desc* d, const void* dy, const void* x, const void
     if (plan.together && products) {
         const int bx = dx ? ax.tiles_m * ax.tiles_n * plan.dx.splits : 0, bw = dw ? aw.tiles_m * aw.tiles_n * plan.dw.splits : 0;
         if constexpr (sizeof(T) == 2) {
-            if (plan.dx.cfg == 1) gemm_pair<T, 128, 128><<<bx + bw + sum_blocks, 256, 0, s>>>(ax, aw, bx, bw, sum);
+            if (plan.dx.cfg == 1) gemm_pair<T, 128, 128><<<bx + bw + sum_blocks, 256, 0, s>>>(ax, aw, bx, bw, sum_blocks, sum);
         }
-        if (plan.dx.cfg == 2) gemm_pair<T, 64, 64><<<bx + bw + sum_blocks, 256, 0, s>>>(ax, aw, bx, bw, sum);
+        if (plan.dx.cfg == 2) gemm_pair<T, 64, 64><<<bx + bw + sum_blocks, 256, 0, s>>>(ax, aw, bx, bw, sum_blocks, sum);
         CVG_LAUNCH_CHECK();
         return sum_slabs<T>(dx ? slab_job<T>(ax, plan.dx) : SlabJob{}, dw ? slab_job<T>(aw, plan.dw) : SlabJob{}, s);
     }
