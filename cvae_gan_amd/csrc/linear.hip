@@ -293,12 +293,15 @@ template <typename T> struct Streams {
 //     of registers, a stage ahead of the LDS: fetching straight to LDS keeps the LDS busy for longer than writing 128 bytes
 //     a cycle does (8192 x 4096 x 4096 dw: staging alone takes 140 us, fragment reads alone 91, both together 221; the
 //     product with its 161 us of MFMAs 322).  dw 237 us (1160 TFLOP/s), dx 260, forward with f32 pre and residual 281.
-//   128 x 128 and 64 x 64: two or three workgroups share a CU and registers are short; direct-to-LDS loads.  Two LDS stages
+//   128 x 128 and 64 x 64: two or three workgroups share a CU; direct-to-LDS loads (550 x 8192 x 528 17 us, 26 by registers).  Two LDS stages
 //     of 32 KB or three of 16: 512 x 4096 x 4096 by small tiles takes 31.9 us with two, 26.9 with three, 27.3 with four,
 //     550 x 8192 x 528 in f32 47.8, 48.7 and 51.5.
-template <int BM> constexpr int ring() { return BM == 64 ? 3 : 2; }
-template <typename T, int BM, int BN> struct TileLds {
-    static constexpr int STAGES = ring<BM>() * (BM + BN) * 128, EPI = 4 * 32 * (BN / 2 * 4 + 16);
+//   Where an operand's rows run along k, bf16 comes by way of registers at every tile: the compiler lets a transposing LDS
+//     read wait for every load to LDS under way (2048 x 2048 x 2048: dx 51 us with, 26 without).
+template <typename T, int BM, bool COL> constexpr bool by_registers() { return BM == 256 || (sizeof(T) == 2 && COL); }
+template <typename T, int BM, bool COL> constexpr int ring() { return BM == 64 && !by_registers<T, BM, COL>() ? 3 : 2; }
+template <typename T, int BM, int BN, bool COL> struct TileLds {
+    static constexpr int STAGES = ring<T, BM, COL>() * (BM + BN) * 128, EPI = 4 * 32 * (BN / 2 * 4 + 16);
     static constexpr int BYTES = STAGES > EPI ? STAGES : EPI;
 };
 struct Yes { static constexpr bool value = true; };
@@ -310,8 +313,8 @@ __device__ __forceinline__ void tile_body(const GemmArgs& a, int id, int slice, 
     typedef Operand<T, BN, NW, BCOL> OB;
     typedef typename Elem<T>::frag frag;
     constexpr int BK = OA::BK, NS = BK / 16;
-    constexpr int STAGE = OA::BYTES + OB::BYTES, D = ring<BM>();
-    constexpr bool REGS = BM == 256;
+    constexpr int STAGE = OA::BYTES + OB::BYTES, D = ring<T, BM, ACOL || BCOL>();
+    constexpr bool REGS = by_registers<T, BM, ACOL || BCOL>();
     constexpr int EP = WN * 4 + 16;                                // epilogue: 32 rows of the wave's columns, f32
     // workgroups go round-robin over the 8 dies, each with its own L2: give every die a run of neighbouring tiles, walked
     // in strips of 4 tile rows
@@ -450,14 +453,21 @@ __device__ __forceinline__ void tile_body(const GemmArgs& a, int id, int slice, 
             __builtin_amdgcn_s_barrier();
             asm volatile("" : : : "memory");
         };
-        fetch_any(0, 0, L);
-        put(0, 0, L);
-        fetch_any(1, 0, L);
-        border();
-        read(0, 0, 0, 0, R);
-        if (1 < stages) put(1, 0, P);
-        fetch_any(2, 0, P);
-        for (; st + 3 < full; ++st, buf ^= 1) {
+        // (The long run has its own beginning: behind a branch it would be unknown how many loads are under way, and the
+        // first write of every stage would wait for all of them, the youngest too.)
+        auto begin = [&](auto long_run) {
+            constexpr bool S = decltype(long_run)::value;
+            if constexpr (S) fetch(Yes{}, 0, L, 0); else fetch_any(0, 0, L);
+            put(0, 0, L);
+            if constexpr (S) fetch(Yes{}, 0, L, 0); else fetch_any(1, 0, L);
+            border();
+            read(0, 0, 0, 0, R);
+            if (S || 1 < stages) put(1, 0, P);
+            if constexpr (S) fetch(Yes{}, 0, P, 0); else fetch_any(2, 0, P);
+        };
+        if (full > 3) {
+          begin(Yes{});
+          for (; st + 3 < full; ++st, buf ^= 1) {
 #pragma unroll
             for (int s = 0; s < NS; ++s) {
                 const bool last = s == NS - 1;
@@ -474,6 +484,9 @@ __device__ __forceinline__ void tile_body(const GemmArgs& a, int id, int slice, 
                         }
                 });
             }
+          }
+        } else {
+            begin(No{});
         }
         for (; st < stages; ++st, buf ^= 1) {
 #pragma unroll
@@ -622,7 +635,7 @@ __device__ __forceinline__ void tile_body(const GemmArgs& a, int id, int slice, 
 
 template <typename T, int BM, int BN, bool ACOL, bool BCOL>
 __global__ void __launch_bounds__(256) gemm_tile(const GemmArgs a) {
-    __shared__ __attribute__((aligned(1024))) char lds[TileLds<T, BM, BN>::BYTES];
+    __shared__ __attribute__((aligned(1024))) char lds[TileLds<T, BM, BN, ACOL || BCOL>::BYTES];
     tile_body<T, BM, BN, ACOL, BCOL>(a, blockIdx.x, blockIdx.y, lds);
 }
 
@@ -749,7 +762,7 @@ struct SumArgs { const float* part; float* out; int P, N; };
 // ahead of the other, so that what starts last is over soonest.
 template <typename T, int BM, int BN>
 __global__ void __launch_bounds__(256) gemm_pair(const GemmArgs dx, const GemmArgs dw, int blocks_dx, int blocks_dw, int blocks_db, const SumArgs db) {
-    __shared__ __attribute__((aligned(1024))) char lds[TileLds<T, BM, BN>::BYTES];
+    __shared__ __attribute__((aligned(1024))) char lds[TileLds<T, BM, BN, true>::BYTES];
     int blk = blockIdx.x - blocks_db;
     if (blk < 0) {
         sum_rows_body(db.part, db.P, db.N, db.out, blockIdx.x, (float (*)[32])lds);
