@@ -562,7 +562,7 @@ Plan plan(const cvg_gn_desc* d, bool backward, bool res) {
     while (nv > unit && (d->HW > cap(nv) || (int64_t)d->B * ceil_div(all, nv) < 256)) nv -= unit;
     const int64_t groups_of = (int64_t)d->B * ceil_div(all, nv);    // workgroups with one tile each
     bool single = d->HW <= cap(nv);
-    if (groups_of < 256 && (int64_t)d->HW * nv > (bf ? 3072 : 1024)) single = false;
+    if (groups_of < 256 && (int64_t)d->HW * nv > (bf ? 3000 : 1000)) single = false;
     p.threads = nv <= 256 ? 256 : 512;
     int rows = rmax;
     if (single) {
