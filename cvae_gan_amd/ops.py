@@ -478,8 +478,9 @@ def _pre(d, pre, x, shape):
 
 
 def linear_act_workspace(x, w, act=ACT_NONE, backward=False):
-    """Workspace (a uint8 tensor) for linear_act_fwd on these operands, with backward also for linear_act_bwd."""
-    d = _linear_desc(x, w, act)
+    """Workspace (a uint8 tensor) for linear_act_fwd on these operands, with backward also for linear_act_bwd (whatever
+    the activation and the type of dw)."""
+    d = _linear_desc(x, w, ACT_SILU if backward else act)
     return _bytes(int(lib.cvg_linear_act_workspace(C.byref(d), int(backward))), x.device)
 
 
@@ -499,7 +500,8 @@ def linear_act_fwd(x, w, y, bias=None, res=None, pre=None, act=ACT_NONE, ws=None
 
 def linear_act_bwd(dy, x, w, pre=None, dx=None, dw=None, dbias=None, act=ACT_NONE, ws=None):
     """Gradients of linear_act_fwd, each optional: dx like x, dw [N, K] (float32 or x's type), dbias f32 [N].  An
-    activation needs the pre of the forward call; the gradient of res is dy itself."""
+    activation needs the pre of the forward call; the gradient of res is dy itself.  dx and a bfloat16 dw are taken with
+    dy act'(pre) rounded to bfloat16, a float32 dw with 16 bits of it (at twice the time of that product)."""
     d = _linear_desc(x, w, act)
     dev, out = x.device, x.shape[:-1] + (d.N,)
     _is("dy", dy, out, x.dtype, dev)
