@@ -336,6 +336,14 @@ def _need(ok, fmt, *args):
         raise CvgError(fmt % args)
 
 
+def _sizes(*sizes):
+    """Sizes on their way into a descriptor's 32-bit fields, which would keep the low half of a larger number."""
+    for n in sizes:
+        if not 0 <= n < 2 ** 31:
+            raise CvgError("size %d does not fit the kernels' 32 bits" % n)
+    return sizes
+
+
 def _is(name, t, shape, dtype, device):
     """t (when given) has this shape, type and device."""
     if t is None or (t.shape == shape and t.dtype == dtype and t.device == device):
@@ -419,7 +427,8 @@ def _gn_desc(x, G, act, eps=0.0):
     for n in shape[1:-1]:
         hw *= n
     _need(act in _ACT_VALUES, "activation %r", act)
-    return GnDesc(_DT[x.dtype], shape[0], hw, shape[-1], int(G), act, 0, 0, 0, 0, 0, eps)
+    _need(G == int(G), "%r groups", G)
+    return GnDesc(_DT[x.dtype], *_sizes(shape[0], hw, shape[-1], int(G)), act, 0, 0, 0, 0, 0, eps)
 
 
 def gn_act_workspace(x, G, backward=False):
@@ -466,7 +475,7 @@ def _linear_desc(x, w, act):
     m = 1
     for n in x.shape[:-1]:
         m *= n
-    return LinearDesc(_DT[x.dtype], m, N, K, act, F32, F32, _pitch("x", x), _pitch("w", w))
+    return LinearDesc(_DT[x.dtype], *_sizes(m, N, K), act, F32, F32, _pitch("x", x), _pitch("w", w))
 
 
 def _pre(d, pre, x, shape):
@@ -535,7 +544,7 @@ def distill_topk(logits, top_val, top_idx, loss, row_loss, dlogits=None, row_wei
     _need(loss.numel() == 1 and loss.dtype == torch.float32 and loss.device == dev, "loss has to be one float32 on %s", dev)
     top_ld = _pitch("top_val", top_val)
     _need((top_ld or top) == (_pitch("top_idx", top_idx) or top), "top_val and top_idx have to share their strides")
-    d = DistillDesc(_DT[logits.dtype], r, logits.shape[-1], top, _pitch("logits", logits), _pitch("dlogits", dlogits), top_ld,
+    d = DistillDesc(_DT[logits.dtype], *_sizes(r, logits.shape[-1], top), _pitch("logits", logits), _pitch("dlogits", dlogits), top_ld,
                     float(temperature), float(grad_scale))
     _launch(lib.cvg_distill_topk, dev, C.byref(d), _p(logits), _p(top_val), _p(top_idx), _p(row_weight), _p(loss),
             _p(row_loss), _p(dlogits))

@@ -1,0 +1,48 @@
+"""What the entry points of group norm, linear layers and distillation have to refuse in the tensor layer, without a GPU."""
+import pytest
+import torch
+
+from test_rowops_refusals import bad
+
+BIG = 2 ** 32 + 5                                        # whose low 32 bits are a small positive number
+
+
+def meta(*shape, dtype=torch.bfloat16):
+    return torch.empty(*shape, dtype=dtype, device="meta")
+
+
+def test_sizes_that_do_not_fit_a_descriptor():
+    """Descriptors hold 32-bit sizes: a larger one must not be cut down to its low half (which a kernel would then take for
+    the size of a small, successful call)."""
+    from cvae_gan_amd import ops
+    f32, i32, need = torch.float32, torch.int32, "32 bits"
+    x, w, y = meta(BIG, 1), meta(8, 1), meta(BIG, 8)
+    bad(lambda: ops.linear_act_fwd(x, w, y), need)
+    bad(lambda: ops.linear_act_bwd(y, x, w, dw=meta(8, 1)), need)
+    bad(lambda: ops.linear_act_workspace(x, w, backward=True), need)
+    bad(lambda: ops.linear_act_fwd(meta(65537, 65537, 8), meta(8, 8), meta(65537, 65537, 8)), need)      # a product of sizes
+    bad(lambda: ops.linear_act_fwd(meta(2, BIG), meta(8, BIG), meta(2, 8)), need)
+    bad(lambda: ops.linear_act_fwd(meta(2, 8), meta(BIG, 8), meta(2, BIG)), need)
+    one = meta(8, dtype=f32)
+    for shape in ((BIG, 8), (1, BIG, 8), (3, 65537, 65537, 8), (1, BIG * 8)):
+        x = meta(*shape)
+        v, st = meta(shape[-1], dtype=f32), meta(2, shape[0], 1, dtype=f32)
+        bad(lambda: ops.gn_act_fwd(x, None, x, 1, None, v, v), need)
+        bad(lambda: ops.gn_act_bwd(x, x, None, meta(*shape), None, 1, st, v, v, v, v), need)
+        bad(lambda: ops.gn_act_workspace(x, 1), need)
+    x = meta(2, 16, 8)
+    bad(lambda: ops.gn_act_fwd(x, None, x, 2 ** 32 + 2, meta(2, 2, 2, dtype=f32), one, one), need)
+    bad(lambda: ops.gn_act_fwd(x, None, x, -2, None, one, one), need)
+    bad(lambda: ops.gn_act_fwd(x, None, x, 2.5, None, one, one), "groups")
+    for rows, v, top in (((BIG,), 4, 2), ((65537, 65537), 4, 2), ((2,), BIG, 2), ((2,), 4, BIG)):
+        bad(lambda: ops.distill_topk(meta(*rows, v), meta(*rows, top, dtype=f32), meta(*rows, top, dtype=i32), meta(1, dtype=f32),
+                                     meta(*rows, dtype=f32)), need)
+
+
+@pytest.mark.parametrize("n", [2 ** 31 - 1, 2 ** 31])
+def test_the_largest_size(n):
+    from cvae_gan_amd import ops
+    if n < 2 ** 31:
+        assert ops._sizes(0, n) == (0, n)
+    else:
+        bad(lambda: ops._sizes(n), "32 bits")
