@@ -11,6 +11,8 @@ stream.  Two groups:
 * tensor-only operators that map one to one onto C entry points without a descriptor struct:
   bn_stats, bn_act_fwd, bn_act_bwd, reparam_kl_fwd, mse_fwd_bwd, adamw, gn_act_fwd, gn_act_bwd,
   linear_act_fwd, linear_act_bwd, distill_topk (arguments as in cvae_gan_amd/ops.py; ws None: allocated).
+  The schemas declare which tensors are written, so an output that is one of the inputs is refused here; the calls of
+  cvae_gan_amd/ops.py that work in place do so there.
 
 They are implemented for the CUDA dispatch key only (ROCm devices dispatch there); there is no
 CPU implementation, so a CPU tensor fails in the dispatcher instead of taking another path."""
@@ -126,15 +128,27 @@ def _adamw(p, g, m, v, lr, beta1, beta2, eps, weight_decay, step):
     ops.adamw(p, g, m, v, p.numel(), lr, beta1, beta2, eps, weight_decay, step)
 
 
+def _apart(name, out, *inputs):
+    """An operator whose schema says that an input is only read must not write it under another name."""
+    if out is not None and out.numel():
+        for t in inputs:
+            if t is not None and t.data_ptr() == out.data_ptr():
+                raise ops.CvgError("torch.ops.cvaegan: %s is an input too; cvae_gan_amd.ops has the call in place" % name)
+
+
 def _gn_act_fwd(x, res, y, groups, stats, gamma, beta, eps, act, ws):
+    _apart("y", y, x, res)
     ops.gn_act_fwd(x, res, y, groups, stats, gamma, beta, eps=eps, act=act, ws=ws)
 
 
 def _gn_act_bwd(dy, x, res, dx, dres, groups, stats, gamma, beta, dgamma, dbeta, act, ws):
+    _apart("dx", dx, dy)
+    _apart("dres", dres, dy)
     ops.gn_act_bwd(dy, x, res, dx, dres, groups, stats, gamma, beta, dgamma, dbeta, act=act, ws=ws)
 
 
 def _linear_act_fwd(x, w, y, bias, res, pre, act, ws):
+    _apart("y", y, res)
     ops.linear_act_fwd(x, w, y, bias=bias, res=res, pre=pre, act=act, ws=ws)
 
 
@@ -143,6 +157,7 @@ def _linear_act_bwd(dy, x, w, pre, dx, dw, dbias, act, ws):
 
 
 def _distill_topk(logits, top_val, top_idx, loss, row_loss, dlogits, row_weight, temperature, grad_scale):
+    _apart("dlogits", dlogits, logits)
     ops.distill_topk(logits, top_val, top_idx, loss, row_loss, dlogits=dlogits, row_weight=row_weight, temperature=temperature,
                      grad_scale=grad_scale)
 

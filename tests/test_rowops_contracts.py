@@ -46,3 +46,31 @@ def test_the_largest_size(n):
         assert ops._sizes(0, n) == (0, n)
     else:
         bad(lambda: ops._sizes(n), "32 bits")
+
+
+def test_torch_operators_keep_to_their_schemas():
+    """torch.ops.cvaegan.* declare their inputs as read only: what ops.py does in place they refuse.  (Called behind the
+    dispatcher, which has no CPU kernel; everything else about the call is right, so that the next refusal is the device's.)"""
+    from cvae_gan_amd import ops, torch_ops as t
+    x, y, z, one, st = torch.zeros(2, 3, 8), torch.zeros(2, 3, 8), torch.zeros(2, 3, 8), torch.ones(8), torch.zeros(2, 2, 1)
+
+    def gn_fwd(y, res=None):
+        t._gn_act_fwd(x, res, y, 1, st, one, one, 1e-5, ops.ACT_SILU, None)
+    bad(lambda: gn_fwd(y), "device tensors")
+    bad(lambda: gn_fwd(x), "y is an input")
+    bad(lambda: gn_fwd(y, res=y), "y is an input")
+
+    def gn_bwd(dx, dres):
+        t._gn_act_bwd(y, x, z, dx, dres, 1, st, one, one, one.clone(), one.clone(), ops.ACT_SILU, None)
+    bad(lambda: gn_bwd(x.clone(), None), "device tensors")
+    bad(lambda: gn_bwd(y, None), "dx is an input")
+    bad(lambda: gn_bwd(x.clone(), y), "dres is an input")
+    w = torch.zeros(8, 8)
+    bad(lambda: t._linear_act_fwd(x, w, y, None, z, None, ops.ACT_NONE, None), "device tensors")
+    bad(lambda: t._linear_act_fwd(x, w, z, None, z, None, ops.ACT_NONE, None), "y is an input")
+    lg, tv, ti = torch.zeros(4, 50), torch.zeros(4, 3), torch.zeros(4, 3, dtype=torch.int32)
+
+    def distill(dl):
+        t._distill_topk(lg, tv, ti, torch.zeros(()), torch.zeros(4), dl, None, 1.0, 1.0)
+    bad(lambda: distill(torch.zeros(4, 50)), "device tensors")
+    bad(lambda: distill(lg), "dlogits is an input")
