@@ -8,8 +8,8 @@ SRCS    := $(SRC_DIR)/api.hip $(SRC_DIR)/igemm.hip $(SRC_DIR)/conv_patch.hip $(S
 OBJS    := $(SRCS:.hip=.o)
 # (the packed f32 instructions stay unused: the compiler forms them from scalar code and some forms have been seen to
 # return wrong values; the host pass does not know the feature and says so)
-FLAGS   := --offload-arch=$(ARCH) -O3 -fPIC -std=c++17 -Wall -Wno-unused-function -Iinclude \
-           -Xclang -target-feature -Xclang -packed-fp32-ops
+UNPACKED := -Xclang -target-feature -Xclang -packed-fp32-ops
+FLAGS   := --offload-arch=$(ARCH) -O3 -fPIC -std=c++17 -Wall -Wno-unused-function -Iinclude $(UNPACKED)
 
 all: $(LIB)
 
@@ -30,8 +30,8 @@ timing: $(LIB)
 	@mkdir -p build_exp
 	$(HIPCC) $(FLAGS) -DEXP_TIMING -c $(SRC_DIR)/conv_patch.hip -o build_exp/conv_patch_timing.o
 	$(HIPCC) --offload-arch=$(ARCH) -shared -fPIC -o build_exp/lib_timing.so build_exp/conv_patch_timing.o $(filter-out %/conv_patch.o,$(OBJS))
-	$(HIPCC) --offload-arch=$(ARCH) -O3 -Wno-unused-value tools/mfma_peak.hip -o build_exp/mfma_peak
-	$(HIPCC) --offload-arch=$(ARCH) -O3 -Wno-unused-value tools/mfma_shape.hip -o build_exp/mfma_shape
+	$(HIPCC) --offload-arch=$(ARCH) -O3 $(UNPACKED) -Wno-unused-value tools/mfma_peak.hip -o build_exp/mfma_peak
+	$(HIPCC) --offload-arch=$(ARCH) -O3 $(UNPACKED) -Wno-unused-value tools/mfma_shape.hip -o build_exp/mfma_shape
 .PHONY: timing
 
 # Host-side sanitizer configuration: the library's host code (validation, planning, launch set-up) compiled with
