@@ -385,7 +385,7 @@ extern "C" int cvg_distill_topk(const cvg_distill_desc* d, const void* logits, c
     CVG_CHECK(d->R >= 0 && d->V >= 1, "distill_topk: R %d, V %d", d->R, d->V);
     CVG_CHECK(d->R <= 0x7fff0000 && d->V <= 0x7ffffff0, "distill_topk: R %d, V %d", d->R, d->V);   // (row loops step past the end)
     CVG_CHECK(d->top >= 1 && d->top <= MAX_TOP, "distill_topk: %d teacher entries (1..%d)", d->top, MAX_TOP);
-    CVG_CHECK(d->temperature >= 1e-37f && d->temperature < INFINITY, "distill_topk: temperature %g", (double)d->temperature);
+    CVG_CHECK(d->temperature >= 1e-37f && d->temperature <= 1e20f, "distill_topk: temperature %g", (double)d->temperature);
     CVG_CHECK((d->logits_ld == 0 || d->logits_ld >= d->V) && (d->dlogits_ld == 0 || d->dlogits_ld >= d->V) &&
               (d->top_ld == 0 || d->top_ld >= d->top), "distill_topk: pitches %d, %d, %d", d->logits_ld, d->dlogits_ld, d->top_ld);
     CVG_CHECK(loss, "distill_topk: null loss");
@@ -404,7 +404,8 @@ extern "C" int cvg_distill_topk(const cvg_distill_desc* d, const void* logits, c
     a.k.hi = (float)k;
     if (d->dtype == CVG_F32 && (double)a.k.hi > k) a.k.hi = nextafterf(a.k.hi, 0.f);
     a.k.lo = (float)(k - (double)a.k.hi);
-    if (!(a.k.lo > 0.f)) a.k.lo = 1e-30f;
+    // (nothing left: any normal number far below hi's last bit; T <= 1e20 keeps both parts of k normal)
+    if (!(a.k.lo > 0.f)) a.k.lo = a.k.hi * 0x1p-40f;
     CVG_CHECK(dlogits != logits || a.ld == a.dld, "distill_topk: in place with different pitches");
     hipStream_t st = (hipStream_t)s;
     if (d->R > 0) {

@@ -1,8 +1,10 @@
 """What the entry points of group norm, linear layers and distillation have to refuse in the tensor layer, without a GPU."""
+import ctypes as C
+
 import pytest
 import torch
 
-from test_rowops_refusals import bad
+from test_rowops_refusals import FAKE, bad, refused
 
 BIG = 2 ** 32 + 5                                        # whose low 32 bits are a small positive number
 
@@ -46,6 +48,16 @@ def test_the_largest_size(n):
         assert ops._sizes(0, n) == (0, n)
     else:
         bad(lambda: ops._sizes(n), "32 bits")
+
+
+@pytest.mark.parametrize("T", [1.1e20, 1e30, 1e38, 3e38])
+def test_distillation_temperatures_beyond_its_exponents(T):
+    """e^(d / T) is taken with log2(e) / T in two f32 parts, which have to be normal numbers.  The low one was 1e-30 where nothing
+    was left for it, more than the high one from T = 1.4e30 on (a logit at f32's lowest value at T = 1e38: 0 in the place of 0.03)."""
+    from cvae_gan_amd._lib import lib, DistillDesc
+    d = DistillDesc()
+    d.dtype, d.R, d.V, d.top, d.temperature, d.grad_scale = 0, 4, 100, 5, T, 1.0
+    assert "temperature" in refused(lib.cvg_distill_topk, C.byref(d), FAKE, FAKE, FAKE, None, FAKE, FAKE, FAKE, None)
 
 
 def test_torch_operators_keep_to_their_schemas():
