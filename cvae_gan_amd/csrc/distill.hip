@@ -407,6 +407,9 @@ extern "C" int cvg_distill_topk(const cvg_distill_desc* d, const void* logits, c
     // (nothing left: any normal number far below hi's last bit; T <= 1e20 keeps both parts of k normal)
     if (!(a.k.lo > 0.f)) a.k.lo = a.k.hi * 0x1p-40f;
     CVG_CHECK(dlogits != logits || a.ld == a.dld, "distill_topk: in place with different pitches");
+    CVG_CHECK(apart({row_loss, dlogits}, {top_val, top_idx, row_weight}) && apart({row_loss}, {logits}) &&
+              apart({loss}, {logits, top_val, top_idx, row_weight, dlogits, d->R > 1 ? row_loss : nullptr}),
+              "distill_topk: an output over another tensor");
     hipStream_t st = (hipStream_t)s;
     if (d->R > 0) {
         if (d->dtype == CVG_BF16) launch<bf16>(a, st); else launch<float>(a, st);

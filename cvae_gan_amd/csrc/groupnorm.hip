@@ -677,6 +677,7 @@ int cvg_gn_act_fwd(const cvg_gn_desc* d, const void* x, const void* res, void* y
     CVG_CHECK(need == 0 || (ws && ws_bytes >= need && ((uintptr_t)ws & 3) == 0), "gn_act_fwd: workspace of %zu bytes, need %zu", ws_bytes, need);
     const int x_ld = d->x_ld ? d->x_ld : d->C, res_ld = d->res_ld ? d->res_ld : d->C, y_ld = d->y_ld ? d->y_ld : d->C;
     CVG_CHECK((y != x || y_ld == x_ld) && (y != res || y_ld == res_ld), "gn_act_fwd: in place with different pitches");
+    CVG_CHECK(apart({y, stats}, {gamma, beta}) && apart({stats}, {x, res}), "gn_act_fwd: an output over another tensor");
     GnArgs a{};
     fill(a, d, p);
     a.x = x; a.res = res; a.y = y; a.stats = stats; a.gamma = gamma; a.beta = beta; a.part = (float*)ws;
@@ -700,7 +701,8 @@ int cvg_gn_act_bwd(const cvg_gn_desc* d, const void* dy, const void* x, const vo
     CVG_CHECK(need == 0 || (ws && ws_bytes >= need && ((uintptr_t)ws & 3) == 0), "gn_act_bwd: workspace of %zu bytes, need %zu", ws_bytes, need);
     const int dy_ld = d->y_ld ? d->y_ld : d->C, dx_ld = d->dx_ld ? d->dx_ld : d->C, dres_ld = d->dres_ld ? d->dres_ld : d->C;
     CVG_CHECK(!dy || ((dx != dy || dx_ld == dy_ld) && (dres != dy || dres_ld == dy_ld)), "gn_act_bwd: in place with different pitches");
-    CVG_CHECK(!dx || (dx != dres && dx != x && dx != res && (!dres || (dres != x && dres != res))),
+    // (dgamma and dbeta are written while other workgroups still read gamma, beta and stats)
+    CVG_CHECK(apart({dx, dres, dgamma, dbeta}, {x, res, stats, gamma, beta}) && apart({dgamma, dbeta}, {dy}),
               "gn_act_bwd: a gradient over another tensor");
     GnArgs a{};
     fill(a, d, p);

@@ -1284,7 +1284,7 @@ int cvg_linear_act_fwd(const cvg_linear_desc* d, const void* x, const void* w, c
     CVG_CHECK((uintptr_t)pre % es_of(d->pre_dtype) == 0 && (uintptr_t)bias % 4 == 0, "linear_act_fwd: misaligned tensor");
     const size_t need = fwd_ws(d);
     CVG_CHECK(need == 0 || (ws && ws_bytes >= need && aligned16(ws)), "linear_act_fwd: workspace of %zu bytes, need %zu", ws_bytes, need);
-    CVG_CHECK(y != x && y != w && y != pre && (!pre || (pre != x && pre != w && pre != res)), "linear_act_fwd: an output over another tensor");
+    CVG_CHECK(apart({y, pre}, {x, w, bias}) && apart({pre}, {res}), "linear_act_fwd: an output over another tensor");
     CVG_CHECK(y != res || ld_of(d->res_ld, d->N) == ld_of(d->y_ld, d->N), "linear_act_fwd: in place with different pitches");
     hipStream_t st = (hipStream_t)s;
     return d->dtype == CVG_BF16 ? forward<bf16>(d, x, w, bias, res, y, pre, (char*)ws, st)
@@ -1305,8 +1305,7 @@ int cvg_linear_act_bwd(const cvg_linear_desc* d, const void* dy, const void* x, 
     CVG_CHECK((uintptr_t)dw % es_of(d->dw_dtype) == 0, "linear_act_bwd: misaligned dw");
     const size_t need = bwd_ws(d);
     CVG_CHECK(need == 0 || (ws && ws_bytes >= need && aligned16(ws)), "linear_act_bwd: workspace of %zu bytes, need %zu", ws_bytes, need);
-    const void* outs[3] = {dx, dw, dbias};
-    for (const void* o : outs) CVG_CHECK(!o || (o != dy && o != x && o != w && o != pre), "linear_act_bwd: a gradient over another tensor");
+    CVG_CHECK(apart({dx, dw, dbias}, {dy, x, w, pre}), "linear_act_bwd: a gradient over another tensor");
     hipStream_t st = (hipStream_t)s;
     if (d->M == 0) return backward_empty(d, dw, dbias, st);
     char* w0 = (char*)ws;

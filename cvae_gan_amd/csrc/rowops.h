@@ -1,5 +1,6 @@
 // Helpers shared by the group-norm, linear and distillation kernels.
 #pragma once
+#include <initializer_list>
 #include "common.h"
 
 // ---- activations (CVG_ACT_*) --------------------------------------------------------------------------------
@@ -79,6 +80,15 @@ __device__ __forceinline__ float wave_max(float v) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
     return v;
+}
+// none of the outputs (null: absent) is one of the inputs or another output
+static inline bool apart(std::initializer_list<const void*> outs, std::initializer_list<const void*> ins) {
+    for (auto o = outs.begin(); o != outs.end(); ++o) {
+        if (!*o) continue;
+        for (const void* i : ins) if (*o == i) return false;
+        for (auto q = outs.begin(); q != o; ++q) if (*q == *o) return false;
+    }
+    return true;
 }
 static inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 

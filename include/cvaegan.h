@@ -515,8 +515,9 @@ int cvg_linear_act_bwd(const cvg_linear_desc* d, const void* dy, const void* x, 
  * An entry whose index lies outside [0, V) is absent (rows with fewer than `top` teacher entries); an index may
  * appear twice.  A row of weight 0, or without an entry of finite value or NaN, has loss and gradient 0 whatever it
  * holds.  row_weight f32 [R] or NULL (ones); row_loss f32 [R]; dlogits (dtype, pitch dlogits_ld) or NULL;
- * dlogits may be logits itself, at the same pitch.  0 <= R <= 0x7fff0000, 1 <= V <= 0x7ffffff0, 1 <= top <= 1024,
- * 1e-37 <= T <= 1e20 (1 / T in two parts are normal f32 numbers); pitches 0 = dense.                          */
+ * dlogits may be logits itself, at the same pitch; no other output may be an input or another output.
+ * 0 <= R <= 0x7fff0000, 1 <= V <= 0x7ffffff0, 1 <= top <= 1024, 1e-37 <= T <= 1e20 (log2(e) / T in two parts are normal
+ * f32 numbers); pitches 0 = dense.                                                                            */
 typedef struct cvg_distill_desc {
     int32_t dtype, R, V, top;
     int32_t logits_ld, dlogits_ld, top_ld;

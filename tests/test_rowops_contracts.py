@@ -4,7 +4,7 @@ import ctypes as C
 import pytest
 import torch
 
-from test_rowops_refusals import FAKE, bad, refused
+from test_rowops_refusals import FAKE, bad, gn, lin, refused
 
 BIG = 2 ** 32 + 5                                        # whose low 32 bits are a small positive number
 
@@ -58,6 +58,35 @@ def test_distillation_temperatures_beyond_its_exponents(T):
     d = DistillDesc()
     d.dtype, d.R, d.V, d.top, d.temperature, d.grad_scale = 0, 4, 100, 5, T, 1.0
     assert "temperature" in refused(lib.cvg_distill_topk, C.byref(d), FAKE, FAKE, FAKE, None, FAKE, FAKE, FAKE, None)
+
+
+def test_small_outputs_over_other_tensors():
+    """Parameter gradients, statistics, losses: an output that is an input, or another output, is written while workgroups still
+    read the other.  (One sample of 2^20 pixels, so that group norm takes its two kernels.)"""
+    from cvae_gan_amd._lib import lib, DistillDesc
+    P = [FAKE + (i << 24) for i in range(12)]
+    d, size = C.byref(gn(B=1, HW=1 << 20)), 1 << 40
+    fwd = dict(x=P[0], res=P[1], y=P[2], stats=P[3], gamma=P[4], beta=P[5])
+    for out, other in (("stats", "gamma"), ("stats", "beta"), ("y", "gamma"), ("y", "beta"), ("stats", "x"), ("stats", "y"), ("stats", "res")):
+        assert "another tensor" in refused(lib.cvg_gn_act_fwd, d, *{**fwd, out: fwd[other]}.values(), P[9], size, None), (out, other)
+    bwd = dict(dy=P[0], x=P[1], res=P[2], dx=P[3], dres=P[4], stats=P[5], gamma=P[6], beta=P[7], dgamma=P[8], dbeta=P[9])
+    for out, others in (("dgamma", set(bwd) - {"dgamma"}), ("dbeta", set(bwd) - {"dbeta"}), ("dx", ("stats", "gamma", "beta")),
+                        ("dres", ("stats", "gamma", "beta"))):
+        for other in others:
+            assert "another tensor" in refused(lib.cvg_gn_act_bwd, d, *{**bwd, out: bwd[other]}.values(), P[10], size, None), (out, other)
+    d = C.byref(lin(M=64))
+    fwd = dict(x=P[0], w=P[1], bias=P[2], res=P[3], y=P[4], pre=P[5])
+    for out in ("y", "pre"):
+        assert "another tensor" in refused(lib.cvg_linear_act_fwd, d, *{**fwd, out: fwd["bias"]}.values(), P[9], size, None), out
+    bwd = dict(dy=P[0], x=P[1], w=P[2], pre=P[3], dx=P[4], dw=P[5], dbias=P[6])
+    for out, other in (("dx", "dw"), ("dw", "dbias"), ("dbias", "dx"), ("dbias", "pre"), ("dbias", "x")):
+        assert "another tensor" in refused(lib.cvg_linear_act_bwd, d, *{**bwd, out: bwd[other]}.values(), P[9], size, None), (out, other)
+    dd = DistillDesc()
+    dd.dtype, dd.R, dd.V, dd.top, dd.temperature = 1, 4, 100, 5, 1.0
+    call = dict(logits=P[0], top_val=P[1], top_idx=P[2], row_weight=P[3], loss=P[4], row_loss=P[5], dlogits=P[6])
+    for out, others in (("loss", set(call) - {"loss"}), ("row_loss", set(call) - {"row_loss"}), ("dlogits", ("top_val", "top_idx", "row_weight"))):
+        for other in others:
+            assert "another tensor" in refused(lib.cvg_distill_topk, C.byref(dd), *{**call, out: call[other]}.values(), None), (out, other)
 
 
 def test_torch_operators_keep_to_their_schemas():
