@@ -513,8 +513,8 @@ int cvg_linear_act_bwd(const cvg_linear_desc* d, const void* dy, const void* x, 
  *   row_loss[r] = row_weight[r] T^2 sum_j p_j (log p_j - log q[idx_j]),  *loss = sum_r row_loss[r],
  *   dlogits[r][i] = grad_scale row_weight[r] T (q_i - sum of p_j with idx_j = i).
  * An entry whose index lies outside [0, V) is absent (rows with fewer than `top` teacher entries); an index may
- * appear twice.  A row of weight 0, or without an entry of finite value or NaN, has loss and gradient 0 whatever it
- * holds.  row_weight f32 [R] or NULL (ones); row_loss f32 [R]; dlogits (dtype, pitch dlogits_ld) or NULL;
+ * appear twice.  A row of weight 0, or none of whose entries is both present and above -inf, has loss and gradient 0
+ * whatever it holds; +inf or NaN among the present entries of another row makes its loss NaN.  row_weight f32 [R] or NULL (ones); row_loss f32 [R]; dlogits (dtype, pitch dlogits_ld) or NULL;
  * dlogits may be logits itself, at the same pitch; no other output may be an input or another output.
  * 0 <= R <= 0x7fff0000, 1 <= V <= 0x7ffffff0, 1 <= top <= 1024, 1e-37 <= T <= 1e20 (log2(e) / T in two parts are normal
  * f32 numbers); pitches 0 = dense.                                                                            */

@@ -238,6 +238,29 @@ def test_distill_more_rows_than_workgroups(ops, dtype, R, V):  # noqa: F811
 
 
 @pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("V", [50, 3000, 70000])
+def test_distill_infinite_entries_of_the_teacher(ops, dtype, V):  # noqa: F811
+    """+inf among a row's entries has no softmax: NaN in its own row.  Where the class is outside it is absent, and -inf alone
+    is a row without entries."""
+    g = torch.Generator(device="cuda").manual_seed(V)
+    inf = float("inf")
+    logits, tv = rnd(g, 7, V, dtype=dtype), rnd(g, 7, 3)
+    ti = torch.stack([torch.randperm(V, generator=g, device="cuda")[:3] for _ in range(7)]).int()
+    tv[0, 1] = inf                                 # beside finite ones
+    tv[1, :] = inf                                 # alone
+    tv[2, 0], tv[2, 1], tv[2, 2] = -inf, inf, -inf
+    tv[3, 0], ti[3, 0] = inf, V                    # absent
+    tv[4, :] = -inf
+    tv[5, 0], w = inf, torch.ones(7, device="cuda")
+    w[5] = 0
+    loss, rl, dl = torch.empty((), device="cuda"), torch.empty(7, device="cuda"), torch.empty_like(logits)
+    ops.distill_topk(logits, tv, ti, loss, rl, dlogits=dl, row_weight=w)
+    assert bool(torch.isnan(rl[:3]).all()) and bool(torch.isfinite(rl[3:]).all())
+    assert float(rl[4]) == 0 and float(rl[5]) == 0 and float(dl[4:6].float().abs().max()) == 0
+    assert bool(torch.isfinite(dl[3:].float()).all()) and bool(torch.isnan(dl[:3].float()).any(1).all())
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
 @pytest.mark.parametrize("V", [600, 1500, 5000, 40000, 70001])
 def test_distill_many_entries_over_many_rows(ops, dtype, V):  # noqa: F811
     """More teacher entries than threads, in rows that follow each other in one workgroup."""
