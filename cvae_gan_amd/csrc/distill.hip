@@ -11,7 +11,9 @@
 // Rows that do not fit (131072 bf16 or 65536 f32 classes) are read twice, the second time mostly from the 256 MB cache.
 // The k teacher entries sit in a hash table in LDS, keyed by the vector of 8 their class falls into; whoever computes
 // that vector's gradient subtracts them and takes their part of the loss, so nothing is gathered or written twice.
-// Bound by memory: 4096 x 131072 bf16 469 us (4.6 TB/s; a copy reaches 5.0-5.4), 2048 x 32768 63 us (4.2 TB/s).
+// Bound by memory.  Call to call over rotating buffers, loss and total included: 4096 x 131072 bf16 472 us (4.55 TB/s; a copy
+// reaches 5.0-5.4), 2048 x 32768 64 us (4.2 TB/s); the kernel alone under the profiler 480 to 540 and 59.  Rows that are
+// no whole number of vectors take branches around their loads and stores: 4096 x 131071 660 us, 2048 x 32003 77.
 #include "rowops.h"
 
 namespace {

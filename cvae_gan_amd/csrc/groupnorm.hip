@@ -7,9 +7,14 @@
 //   one tile per (sample, slab): the workgroup normalises its registers and writes y; x is read once.
 //   more than one: the tiles write (mean, M2) per group, a second kernel merges them (Chan's formula) and applies.
 // The backward pass is built the same way over per-channel sums of g and g * xhat, which also give dgamma / dbeta.
-// Bound by memory.  bf16, kernels alone: 256 x 32 x 32 x 128 with skip forward 35 us (200 MB); 256 x 64 x 64 x 64 forward
-// 75 us (3.6 TB/s) and backward 143 (2.8 TB/s: x and dy of one workgroup fill a CU's registers, so its loads, sums and
-// stores take turns; workgroups that walk over samples and load ahead were slower, 232 against 217 us for both).
+// Bound by memory.  bf16: 256 x 32 x 32 x 128 with skip forward 46.6 us call to call over rotating buffers (201 MB, 4.3 TB/s; 35
+// where the 256 MB cache still holds them); 256 x 64 x 64 x 64 forward 75-78 us (3.5 TB/s; 128 registers a thread, two
+// workgroups a CU, which costs 48 to 68 bytes of scratch memory a lane) and backward 143-146 (2.8 TB/s: x and dy of one
+// workgroup fill a CU's registers, so its loads, sums and stores take turns; workgroups that walk over samples and load ahead
+// were slower, 232 against 217 us for both).
+// In the tiled form every workgroup merges the partial sums of its whole sample, work that grows with the square of the
+// tiles: one picture of 64 channels, forward / backward, takes 57 / 64 us at 512 x 512, 144 / 235 at 1024 x 1024 (704 tiles
+// at 600 x 600), 902 / 1895 at 2048 x 2048, where the tensors need 206 / 310.
 #include "rowops.h"
 
 namespace {
@@ -184,7 +189,7 @@ __global__ void __launch_bounds__(MAXT, WAVES) gn_fwd_tile(const GnArgs a) {
     const Place p = gn_place(a, blockIdx.x);
     const size_t row0 = (size_t)p.b * a.HW + p.r0;
     const int rows = p.r1 - p.r0, c = p.c0 + (p.live ? p.chunk * 8 : 0);
-    float ga[8], be[8];                              // before the tile: what they wait for is short
+    float ga[8], be[8];                              // (before the tile: what they wait for is short; part of them is spilled at 16 chunks)
     load8<float>(a.gamma + c, ga);
     load8<float>(a.beta + c, be);
     const T* xp = (const T*)a.x + row0 * a.x_ld + c;
@@ -546,8 +551,13 @@ int check(const cvg_gn_desc* d, const char* who) {
 //     forward on 256 x 32 x 32 x 128 bf16 with skip: 47 us at 64-byte slabs, 53 at 128 (too few workgroups), and on
 //     256 x 64 x 64 x 64 (512 KB a sample, so 32-byte slabs) 76 us against 87 for the two kernels of the tiled form.
 //   Few samples: a workgroup's own arithmetic counts, about 1.8 us per 1000 bf16 chunks (5 in f32), against some 5 us
-//     for a second launch: one 64 x 64 x 64 picture takes 11.4 us as 8 tiles of 4096 chunks and 9.2 as 64 of 512, the
-//     f32 crop 3 x 1961 x 72 13.9 forward and 17.7 backward as 27 tiles and 10.0 and 12.6 as 216.
+//     for a second launch.  Forward / backward us of 64 channels in 32 groups, one workgroup per slab and in tiles:
+//       bf16, 1 sample    1024 pixels 6.4 / 10.4 and 8.2 / 9.1   2025  9.4 / 14.7 and  8.3 /  8.4   4096 13.5 / 22.9 and  8.4 /  9.0
+//             8 samples   2025        8.9 / 14.0 and 10.2 / 11.9 3025 12.0 / 18.5 and 14.1 / 18.1   4096 13.0 / 20.8 and 12.4 / 14.9
+//       f32,  1 sample     784        7.0 / 10.3 and 8.7 / 9.7   1024  7.2 / 12.4 and  8.6 /  9.8   2025 11.4 / 18.0 and  8.8 /  9.0
+//             8 samples   1024        8.4 / 12.5 and 10.3 / 12.4 1444 10.1 / 15.4 and 12.6 / 15.8   2025 11.6 / 17.9 and 11.9 / 13.3
+//     One 64 x 64 x 64 picture is 16 tiles of 256 chunks in each of 8 slabs, the f32 crop 3 x 1961 x 72 (10.3 forward, 12.7
+//     backward) 8 tiles in each of 27.
 Plan plan(const cvg_gn_desc* d, bool backward, bool res) {
     Plan p;
     const int cg = d->C / d->G, unit = cg / gcd(cg, 8);             // chunks of 8 channels that hold whole groups

@@ -292,7 +292,7 @@ template <typename T> struct Streams {
 //     128 sums of eight waves need 6 for 8, and then the LDS is busy as long as the matrix units).  Its operands come by way
 //     of registers, a stage ahead of the LDS: fetching straight to LDS keeps the LDS busy for longer than writing 128 bytes
 //     a cycle does (8192 x 4096 x 4096 dw: staging alone takes 140 us, fragment reads alone 91, both together 221; the
-//     product with its 161 us of MFMAs 322).  dw 237 us (1160 TFLOP/s), dx 260, forward with f32 pre and residual 281.
+//     product with its 161 us of MFMAs 322).  dw 250 us (1100 TFLOP/s; 237 at best), dx 262, forward with f32 pre and residual 284.
 //   128 x 128 and 64 x 64: two or three workgroups share a CU; direct-to-LDS loads (550 x 8192 x 528 17 us, 26 by registers).  Two LDS stages
 //     of 32 KB or three of 16: 512 x 4096 x 4096 by small tiles takes 31.9 us with two, 26.9 with three, 27.3 with four,
 //     550 x 8192 x 528 in f32 47.8, 48.7 and 51.5.
@@ -992,6 +992,8 @@ int check(const cvg_linear_desc* d, const char* who) {
 // cycle chip-wide) and a launch.  Forward bf16, us by 256 x 256 / 128 x 128 / 64 x 64 tiles:
 //   4096 x 4096 x 4096  116 / 131 / 203    2048 x 2048 x 2048  46 / 28 / 29    8192 x 1024 x 1024  35 / 23 / 29
 //   3000 x 3000 x 1000   39 /  41 /  46     512 x 4096 x 4096  45 / 35 / 27     550 x 8192 x  528  26 / 15 / 16
+// (The estimate counts two workgroups of 64 x 64 tiles a CU, where three run since their LDS has three stages: counting
+// three left the times of these sizes, of 1000 x 1000 x 2056, 256 x 8192 x 1024 and of f32 as they are.)
 // f32, whose MFMAs take eight times as long and need no more bytes, always takes 64 x 64: 128 x 128 measured 1114 against
 // 986 us at 4096 x 4096 x 4096, 217 against 148 at 3000 x 3000 x 1000.
 struct Tile { int cfg, splits, k_split; double t; };

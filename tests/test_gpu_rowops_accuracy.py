@@ -55,3 +55,25 @@ def test_f32_weight_gradient_of_infinite_gradients(ops):  # noqa: F811
     ops.linear_act_bwd(dy, x, w, pre=pre, dw=dw, act=ops.ACT_LRELU)
     rest = [i for i in range(16) if i not in (5, 9)]
     assert bool((dw[5] == float("inf")).all()) and bool(torch.isnan(dw[9]).all()) and bool(torch.isfinite(dw[rest]).all())
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_f32_sums_of_bf16_data(ops, act):  # noqa: F811
+    """Parameter gradients are f32 sums of unrounded terms.  Their activations' derivatives come from v_exp_f32 and v_rcp_f32 as
+    they are: off by some 4 u (1 + |v|) each, against terms of about half of |dy|, 2e-6 of the terms' norm at |v| <= 3; the
+    sums' own roundings and those of xhat add less."""
+    from test_gpu_rowops import gn_ref
+    g = torch.Generator(device="cuda").manual_seed(3)
+    for B, HW, C, G in ((64, 1024, 128, 32), (2, 16384, 64, 32)):
+        x, dy, gamma, beta = rnd(g, B, HW, C, dtype=BF, scale=1.5, mean=0.3), rnd(g, B, HW, C, dtype=BF), rnd(g, C, mean=1.0, scale=0.2), rnd(g, C, scale=0.2)
+        ref = gn_ref(x, None, gamma, beta, G, 1e-5, act, dy)
+        y, dx, stats, dg, db = torch.empty_like(x), torch.empty_like(x), torch.empty(2, B, G, device="cuda"), torch.empty_like(gamma), torch.empty_like(gamma)
+        ops.gn_act_fwd(x, None, y, G, stats, gamma, beta, act=ops.ACTS[act])
+        ops.gn_act_bwd(dy, x, None, dx, None, G, stats, gamma, beta, dg, db, act=ops.ACTS[act])
+        assert off(dg, ref["dgamma"]) < 5e-6 and off(db, ref["dbeta"]) < 5e-6
+    M, N, K = 4096, 512, 64
+    x, w, dy, pre = rnd(g, M, K, dtype=BF), rnd(g, N, K, dtype=BF), rnd(g, M, N, dtype=BF), rnd(g, M, N)
+    db = torch.empty(N, device="cuda")
+    ops.linear_act_bwd(dy, x, w, pre=pre, dbias=db, act=ops.ACTS[act])
+    ref = (dy.double() * act64(pre.double(), act)[1]).sum(0)
+    assert off(db, ref) < 5e-6
