@@ -1006,9 +1006,14 @@ Tile choose_split(int dtype, int c, int64_t M, int64_t N, int64_t K) {
     const int64_t stages = (K + bk - 1) / bk;
     Tile best{c, 1, (int)round_up(K, bk), 1e300};
     const int64_t tiles = ((M + sh.bm - 1) / sh.bm) * ((N + sh.bn - 1) / sh.bn);
-    for (int64_t sp = 1; sp <= 64; sp *= 2) {
+    // The bf16 matrix instruction cuts off what lies below the last bits of a sum that has grown large beside its products, and
+    // cuts downwards, by some 1e-3 of the sum's last bit each: of K terms in ranges of L, sqrt(K L) times 1 to 3e-12 of the norm.  2^28 rows
+    // in 64 ranges put every element of dw too low, by 1e-4; at most 2^18 terms a range hold that to 2e-5 there and to 1e-6 at
+    // 2^20 rows.  (f32 sums start again every 512 k.)
+    const int64_t most = dtype == CVG_BF16 ? (1 << 18) / bk : stages, least = (stages + most - 1) / most;
+    for (int64_t sp = least; sp == least || sp <= 64; sp *= 2) {
         const int64_t per = (stages + sp - 1) / sp;
-        if (sp > 1 && (per < 2 || tiles * sp > 2048)) break;
+        if (sp > least && (per < 2 || tiles * sp > 2048)) break;
         const int64_t real = (stages + per - 1) / per;                 // ranges that hold any k
         const int64_t wgs = tiles * real, per_cu = (wgs + 255) / 256;
         const int64_t rounds = (per_cu + sh.occ - 1) / sh.occ;
