@@ -221,11 +221,19 @@ __global__ void __launch_bounds__(TPR == 64 ? 256 : TPR, 4) distill_row(const Di
                 }
             }
         } else {
-            for (int i = tid; i < nvec; i += TPR) {
-                float v[8];
-                vec_load<T>(row, off, a.V, i, v);
-                run.add(v, k);
+            // 64 vectors at a time: in one sum of thousands (2^31 classes: 262144) terms below its last bit would all be lost,
+            // 7e-4 of the whole where a thread's first vector holds the largest logit
+            Running<T> whole = run;
+            for (int i = tid; i < nvec;) {
+                for (int n = 0; n < 64 && i < nvec; ++n, i += TPR) {
+                    float v[8];
+                    vec_load<T>(row, off, a.V, i, v);
+                    run.add(v, k);
+                }
+                whole.join(run.m, run.s, k);
+                run = Running<T>{-3.402823466e38f, 0.f};
             }
+            run = whole;
         }
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) run.join(__shfl_xor(run.m, o, 64), __shfl_xor(run.s, o, 64), k);

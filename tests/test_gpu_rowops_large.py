@@ -96,6 +96,32 @@ def test_linear_of_the_widest_rows(ops, dtype, size):  # noqa: F811
     assert off(dw, dy.double().t().contiguous() @ x.double()) < 2e-6
 
 
+@pytest.mark.parametrize("V", [0x7ffffff0, 0x7fffffe9])
+def test_distill_of_the_most_classes(ops, V):  # noqa: F811
+    """One row of 2^31 - 16 bf16 logits in place, zero but for its ends.  A thread's 262144 vectors are added 64 at a time:
+    within 64 of them e^-20 each gets lost beside a spike (64 x 8 x 2e-9), then 4096 + 22 roundings of u / sqrt(3) in the mean
+    square, 2.2e-6 together: 1e-5 allowed."""
+    logits = torch.zeros(1, V, dtype=BF, device="cuda")
+    for i in (0, V - 1):
+        logits[0, i] = 20.0
+    ti = torch.tensor([[0, V - 1, 5, 1 << 30, V - 9]], dtype=torch.int32, device="cuda")
+    tv = torch.tensor([[1.0, 2.0, 0.5, 0.25, 0.125]], device="cuda")
+    loss, rl = torch.empty((), device="cuda"), torch.empty(1, device="cuda")
+    ops.distill_topk(logits, tv, ti, loss, rl, dlogits=logits, grad_scale=1e6)
+    z = V - 2 + 2 * math.exp(20.0)
+    p = torch.softmax(tv[0].double(), 0).tolist()
+    lq = [20.0 - math.log(z)] * 2 + [-math.log(z)] * 3
+    want = sum(q * (math.log(q) - l) for q, l in zip(p, lq))
+    assert abs(float(rl) - want) < 1e-5 * want and float(loss) == float(rl)
+    rest = 1e6 / z
+    for c, q, l in zip(ti[0].tolist(), p, lq):
+        g = 1e6 * (math.exp(l) - q)
+        assert abs(float(logits[0, c]) - g) < 2.0 ** -8 * abs(g) + 1e-4
+        logits[0, c] = rest
+    least, most = torch.aminmax(logits)
+    assert abs(float(least) - rest) < 2.0 ** -8 * rest and float(most) == float(least)
+
+
 def test_distill_of_more_than_2_31_logits(ops):  # noqa: F811
     R, V, k, g = 2200000, 1000, 5, gen(5)
     logits = torch.randn(R, V, generator=g, device="cuda", dtype=BF)
