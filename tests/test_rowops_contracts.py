@@ -60,6 +60,20 @@ def test_distillation_temperatures_beyond_its_exponents(T):
     assert "temperature" in refused(lib.cvg_distill_topk, C.byref(d), FAKE, FAKE, FAKE, None, FAKE, FAKE, FAKE, None)
 
 
+def test_workspaces_of_the_more_exact_weight_gradient():
+    """dw in f32 behind an activation needs more than dw in bf16; what Python allocates serves every activation and type."""
+    from cvae_gan_amd import ops
+    from cvae_gan_amd._lib import lib
+    M, N, K = 512, 256, 128
+    need = {(act, dt): lib.cvg_linear_act_workspace(C.byref(lin(M=M, N=N, K=K, act=act, dw_dtype=dt)), 1) for act in (0, 2) for dt in (0, 1)}
+    assert need[2, 0] > need[2, 1] == need[0, 0] == need[0, 1]
+    d = C.byref(lin(M=M, N=N, K=K, act=2, dw_dtype=0))
+    P = [FAKE + (i << 24) for i in range(8)]
+    assert "workspace" in refused(lib.cvg_linear_act_bwd, d, *P[:7], P[7], need[2, 1], None)
+    x, w = torch.zeros(M, K, dtype=torch.bfloat16), torch.zeros(N, K, dtype=torch.bfloat16)
+    assert ops.linear_act_workspace(x, w, backward=True).numel() == need[2, 0]
+
+
 def test_small_outputs_over_other_tensors():
     """Parameter gradients, statistics, losses: an output that is an input, or another output, is written while workgroups still
     read the other.  (One sample of 2^20 pixels, so that group norm takes its two kernels.)"""
